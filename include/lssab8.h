@@ -49,7 +49,9 @@ enum {
   LSSAB8_DEV_EV_RANGE = 1,  /* e_v outside [-32, 40]: reference/lssab9_torch.py:158 assert    */
   LSSAB8_DEV_TIMEOUT = 2,   /* a bounded pipeline wait gave up                                */
   LSSAB8_DEV_BAD_PAGE = 4,  /* a block-table entry outside [0, num_pages)                     */
-  LSSAB8_DEV_ALIGN = 8      /* lssab8_kv_append: a source row not on a 16-byte boundary        */
+  LSSAB8_DEV_ALIGN = 8,     /* lssab8_kv_append: a source row not on a 16-byte boundary        */
+  LSSAB8_DEV_PLAN = 16      /* request lengths that do not fit their buffers or the 128-row
+                               grid, or sequences that do not share the prefix they were given  */
 };
 
 /* Library identity: writes "lssab8-b200 <version> T2=<sha256 of the T2 csv>" (NUL-terminated)
@@ -266,6 +268,78 @@ int lssab8_decode_noalloc(const void* q, int dtype, const int64_t* qs, int B, in
                           const int8_t* k8p, const int8_t* v8p, const int32_t* ek, const int32_t* ev,
                           const int32_t* ev0, int max_blocks, int split_blocks, int sink, void* out, int out_dtype,
                           const int64_t* os, void* stream);
+
+/* -------------------------------------------------------------- serving-step operators
+ * No counterparts in the reference, whose engine (a separate codebase) does these in its own code;
+ * the attention forms compute the same contract rows as the entry points above. */
+
+/* Rotary positions.  x [B, H, T, dh] (strides xs) -> y, same type: the first rot (even) channels of every row
+ * are turned by the row's position, the others copied.  Pair i < rot / 2 is channels (i, i + rot / 2)
+ * (layout 0) or (2 i, 2 i + 1) (layout 1), its angle freq[i] / 2^64 turns a position: an exact integer
+ * product, so far positions lose nothing.  (x1, x2) -> factor (x1 cos - x2 sin, x2 cos + x1 sin) in binary32,
+ * rounded once; inverse = 1 negates the sine: the transposed map, hence the gradient.  positions: int64
+ * (pos64 = 1) or int32, the position of token (b, t) at element b*ps[0] + t*ps[1].  y may be x (same
+ * strides); any other overlap is not allowed.  dh <= 512, any alignment. */
+int lssab8_rotate(const void* x, int dtype, int B, int H, int T, int dh, const int64_t* xs, const void* positions,
+                  int pos64, const int64_t* ps, const uint64_t* freq, float factor, int rot, int layout, int inverse,
+                  void* y, const int64_t* ys, void* stream);
+
+/* A step's new tokens in one launch: q [N, H, dh] rotated into q_out (may be q), k [N, KVH, dh] rotated and
+ * v copied into the engine's paged float cache, k_cache / v_cache [num_pages, 16, KVH, dh] (strides kcs / vcs of
+ * the first three dimensions, channels contiguous) in cache_dtype, at slot page * 16 + row.  Slot -1 (the padded
+ * end of a step) stores nothing; any other slot outside the cache sets LSSAB8_DEV_BAD_PAGE and stores nothing.
+ * Two tokens with one slot: either is stored.  qs / ks / vs / os: token and head strides, channels contiguous. */
+int lssab8_rotate_append(const void* q, const void* k, const void* v, int dtype, int N, int H, int KVH, int dh,
+                         const int64_t* qs, const int64_t* ks, const int64_t* vs, const void* positions, int pos64,
+                         int64_t pos_stride, const uint64_t* freq, float factor, int rot, int layout, void* q_out,
+                         const int64_t* os, void* k_cache, void* v_cache, int cache_dtype, const int64_t* kcs,
+                         const int64_t* vcs, int num_pages, const int64_t* slots, void* stream);
+
+/* A step's tables on the device.  Sequence i grows from before[i] to before[i] + fresh[i] tokens.  Its new
+ * 16-token pages are the next entries of free_pages, in sequence order, and are written to its row of block_table
+ * [n, max_pages] (row stride table_stride; other entries are left as they were).  query_start_loc [n + 1]:
+ * exclusive sums of fresh; seq_lens [n]: lengths after; for each new token, in sequence order, slot_mapping =
+ * page * 16 + row, positions and seq_index; entries of the [cap] arrays past the last token get -1, 0 and -1.
+ * pages_used [1]: entries of free_pages taken.  Lengths that do not fit (negative, over 2^30, more tokens than cap,
+ * more pages than nfree or max_pages, a missing page in the table) set LSSAB8_DEV_PLAN; the tokens concerned get
+ * slot -1.  n <= 16384.  seq_lens may not be before. */
+int lssab8_step_tables(const int32_t* before, const int32_t* fresh, int n, int32_t* block_table, int64_t table_stride,
+                       int max_pages, const int32_t* free_pages, int nfree, int cap, int32_t* query_start_loc,
+                       int32_t* seq_lens, int64_t* slot_mapping, int64_t* positions, int32_t* seq_index,
+                       int32_t* pages_used, void* stream);
+
+/* Bytes of workspace lssab8_prefill_paged needs. */
+size_t lssab8_prefill_paged_workspace_size(int N, int H, int KVH, int dh, int B);
+
+/* All prompt rows of a step in one call, over the paged lattice (which already holds their keys).  Sequence b's
+ * rows of q [N, H, dh] are [cu_q[b], cu_q[b + 1]) and stand at its last positions, [T0, seq_lens[b]), T0 a multiple
+ * of 128 (the contract's chunk rule).  A row at position i sees the keys of its own sequence (document mask)
+ * up to i or, when i < prefix_lens[b], up to prefix_lens[b] - 1 (prefix mask; prefix_lens NULL: none), and is the
+ * contract's row over these keys: without a prefix, bit-identical to lssab8_prefill of the sequence alone.
+ * active [B] (NULL: all): sequences with 0 have no rows here.  Rows of q that belong to no such sequence, and
+ * sequences that break a rule (LSSAB8_DEV_PLAN / LSSAB8_DEV_BAD_PAGE), leave out as it was.  out [N, H, dh].
+ * Lattice arguments as in lssab8_decode; any group; dh in {64, 128}. */
+int lssab8_prefill_paged(const void* q, int dtype, const int64_t* qs, int N, int H, int KVH, int dh, const int32_t* cu_q,
+                         const int32_t* seq_lens, const int32_t* prefix_lens, const uint8_t* active, int B,
+                         const int32_t* block_table, int max_pages, int num_pages, const int8_t* k8p,
+                         const int8_t* v8p, const int32_t* ek, const int32_t* ev, const int32_t* ev0, int max_blocks,
+                         int sink, void* out, int out_dtype, const int64_t* os, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Bytes of workspace lssab8_decode_shared needs (0: refused shape). */
+size_t lssab8_decode_shared_workspace_size(int B, int H, int KVH, int dh, int max_blocks, int shared_len);
+
+/* lssab8_decode for a batch whose sequences share their first shared_len tokens (>= 128): the first shared_len /
+ * 128 blocks are the same pages with the same exponents in every live sequence, and are read and
+ * scored once for all of them.  Same rows, bit for bit, as lssab8_decode.  A sequence of length 0 is not live and
+ * its rows of out stay as they were; one shorter than the shared blocks sets LSSAB8_DEV_PLAN and is left out; one
+ * whose shared pages or exponents differ from the first live sequence's sets LSSAB8_DEV_PLAN (its rows hold
+ * the first sequence's prefix). */
+int lssab8_decode_shared(const void* q, int dtype, const int64_t* qs, int B, int H, int KVH, int dh,
+                         const int32_t* seq_lens, int shared_len, const int32_t* block_table, int max_pages,
+                         int num_pages, const int8_t* k8p, const int8_t* v8p, const int32_t* ek, const int32_t* ev,
+                         const int32_t* ev0, int max_blocks, int sink, void* out, int out_dtype, const int64_t* os,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------- self-test */
 

@@ -10,7 +10,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIBPATH = os.path.join(_HERE, "liblssab8_b200.so")
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
-DEV_EV_RANGE, DEV_TIMEOUT, DEV_BAD_PAGE, DEV_ALIGN = 1, 2, 4, 8
+DEV_EV_RANGE, DEV_TIMEOUT, DEV_BAD_PAGE, DEV_ALIGN, DEV_PLAN = 1, 2, 4, 8, 16
 
 # every symbol include/lssab8.h declares (tests check the library exports each one)
 SYMBOLS = (
@@ -21,7 +21,9 @@ SYMBOLS = (
     "lssab8_prefill_chunk_lattice", "lssab8_prefill_workspace_size", "lssab8_prefill",
     "lssab8_prefill_peers", "lssab8_peer_export", "lssab8_peer_import", "lssab8_peer_close", "lssab8_peer_copy2d",
     "lssab8_decode_prep_kv", "lssab8_kv_append", "lssab8_decode_workspace_size", "lssab8_decode",
-    "lssab8_decode_noalloc", "lssab8_selftest_div", "lssab8_selftest_rescale", "lssab8_selftest_timeout",
+    "lssab8_decode_noalloc", "lssab8_rotate", "lssab8_rotate_append", "lssab8_step_tables",
+    "lssab8_prefill_paged_workspace_size", "lssab8_prefill_paged", "lssab8_decode_shared_workspace_size",
+    "lssab8_decode_shared", "lssab8_selftest_div", "lssab8_selftest_rescale", "lssab8_selftest_timeout",
 )
 
 _lib = None
@@ -70,6 +72,18 @@ def load():
     L.lssab8_decode_workspace_size.restype = SZ
     L.lssab8_decode.argtypes = [P, I, PI64, I, I, I, I, P, P, I, I, P, P, P, P, P, I, I, I, P, I, PI64, P, SZ, P]
     L.lssab8_decode_noalloc.argtypes = [P, I, PI64, I, I, I, I, P, P, I, I, P, P, P, P, P, I, I, I, P, I, PI64, P]
+    F = ctypes.c_float
+    L.lssab8_rotate.argtypes = [P, I, I, I, I, I, PI64, P, I, PI64, P, F, I, I, I, P, PI64, P]
+    L.lssab8_rotate_append.argtypes = [P, P, P, I, I, I, I, I, PI64, PI64, PI64, P, I, I64, P, F, I, I, P, PI64, P, P, I,
+                                       PI64, PI64, I, P, P]
+    L.lssab8_step_tables.argtypes = [P, P, I, P, I64, I, P, I, I, P, P, P, P, P, P, P]
+    L.lssab8_prefill_paged_workspace_size.argtypes = [I] * 5
+    L.lssab8_prefill_paged_workspace_size.restype = SZ
+    L.lssab8_prefill_paged.argtypes = [P, I, PI64, I, I, I, I, P, P, P, P, I, P, I, I, P, P, P, P, P, I, I, P, I, PI64, P,
+                                       SZ, P]
+    L.lssab8_decode_shared_workspace_size.argtypes = [I] * 6
+    L.lssab8_decode_shared_workspace_size.restype = SZ
+    L.lssab8_decode_shared.argtypes = [P, I, PI64, I, I, I, I, P, I, P, I, I, P, P, P, P, P, I, I, P, I, PI64, P, SZ, P]
     L.lssab8_selftest_div.argtypes = [P, P, I64, P, P]
     L.lssab8_selftest_rescale.argtypes = [P, P, I64, P, P]
     L.lssab8_selftest_timeout.argtypes = [P] * 6 + [I] * 7 + [P, PI64, P]

@@ -49,7 +49,8 @@ def check_device_errors(device=None):
     if bits & _lib.DEV_EV_RANGE:
         raise AssertionError("e_v outside the contract clamp")
     if bits:
-        raise RuntimeError("LSSA-B8 device error bits 0x%x (timeout=2, bad page=4, misaligned row=8)" % bits)
+        raise RuntimeError("LSSA-B8 device error bits 0x%x (timeout=2, bad page=4, misaligned row=8, "
+                           "request lengths or prefixes that do not fit=16)" % bits)
 
 
 _WS = {}

@@ -1,7 +1,7 @@
 """Build liblssab8_b200.so in place (nvcc, sm_100a only).
 
-The library is one translation unit (csrc/capi.cu includes the kernel headers).  Floating-point
-flags are part of the contract, not tuning: no fast math, no FMA contraction, IEEE division and
+The library is two translation units, compiled side by side: csrc/capi.cu (quantisers, prefill,
+decode) and csrc/serving.cu (the serving-step operators).  Floating-point flags are part of the contract, not tuning: no fast math, no FMA contraction, IEEE division and
 denormals, so every binary32 operation in the fold is the single RN operation the contract names.
 """
 import os
@@ -11,12 +11,14 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblssab8_b200.so")
-SOURCES = ["capi.cu", "common.cuh", "tcgen05.cuh", "prep.cuh", "prefill.cuh", "decode.cuh", "decode_tc.cuh", "t2_table.inc"]
+UNITS = ["capi.cu", "serving.cu"]
+SOURCES = UNITS + ["common.cuh", "host.cuh", "tcgen05.cuh", "prep.cuh", "prefill.cuh", "decode.cuh", "decode_tc.cuh",
+                   "rotary.cuh", "tables.cuh", "paged.cuh", "t2_table.inc"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-ftz=false", "-prec-div=true", "-prec-sqrt=true", "-fmad=false",
 ]
 
@@ -39,13 +41,20 @@ def stale():
 def build(force=False, verbose=False):
     if not force and not stale():
         return LIB
-    cmd = [nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB, os.path.join(CSRC, "capi.cu")]
-    r = subprocess.run(cmd, cwd=CSRC, capture_output=True, text=True)
-    if r.returncode != 0:
-        sys.stderr.write(r.stdout + r.stderr)
+    objs = [os.path.join(HERE, u.replace(".cu", ".o")) for u in UNITS]
+    cmds = [[nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", o, os.path.join(CSRC, u)]
+            for u, o in zip(UNITS, objs)]
+    jobs = [subprocess.Popen(c, cwd=CSRC, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for c in cmds]
+    logs = [j.communicate()[0] for j in jobs]
+    if all(j.returncode == 0 for j in jobs):
+        r = subprocess.run([nvcc(), "-shared", "-o", LIB] + NVCC_FLAGS[:2] + objs, cwd=CSRC, capture_output=True, text=True)
+        logs.append(r.stdout + r.stderr)
+        jobs.append(r)
+    if any(j.returncode != 0 for j in jobs):
+        sys.stderr.write("".join(logs))
         raise RuntimeError("nvcc failed building liblssab8_b200.so")
     if verbose:
-        sys.stderr.write(r.stderr)
+        sys.stderr.write("".join(logs))
     return LIB
 
 

@@ -3,19 +3,12 @@
 // Host-side responsibilities: argument validation (every error is a status code, never an
 // exception), TMA tensor-map encoding, workspace carving, kernel instantiation by
 // (head dim, sink, output dtype), and the per-device error word.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-#include <cuda_runtime.h>
-
 #include <cstdio>
-#include <algorithm>
-#include <utility>
 #include <cstring>
 #include <mutex>
 
 #include "../../include/lssab8.h"
-#include "common.cuh"
-#include "prep.cuh"
+#include "host.cuh"
 #include "prefill.cuh"
 #include "decode.cuh"
 #include "decode_tc.cuh"
@@ -29,15 +22,12 @@ constexpr const char* kVersion = "0.1.0";
 // ------------------------------------------------------------------ device error word
 __device__ int g_dev_err;
 
-struct DevState {
-  int* err = nullptr;
-  bool prefill_attr_set = false;
-  int num_sms = 0;
-};
 std::mutex g_mu;
 DevState g_dev[64];
 
-int dev_state(DevState** out) {
+}  // namespace
+
+int lssab8::dev_state(DevState** out) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kErrCuda;
   std::lock_guard<std::mutex> lk(g_mu);
@@ -54,53 +44,20 @@ int dev_state(DevState** out) {
 }
 
 // ------------------------------------------------------------------ TMA encode (driver API)
-PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-
-int get_encode() {
+PFN_cuTensorMapEncodeTiled_v12000 lssab8::encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
-  static int rc = kOk;
   std::call_once(once, [] {
-    void* fn = nullptr;
+    void* f = nullptr;
     cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess || !fn) {
-      rc = kErrCuda;
-      return;
-    }
-    g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
   });
-  return rc;
+  return fn;
 }
 
-// rows x dh int8 matrix, box 128 rows x dh, swizzle = dh bytes
-// 2-D int8 tensor map over [rows, dh] (row pitch dh bytes), boxes of box_rows x dh, swizzled for
-// the UMMA K-major layouts (128B swizzle at dh 128, 64B at dh 64).
-int make_tmap(CUtensorMap* tm, const void* base, long long rows, int dh, int box_rows = 128) {
-  if (get_encode() != kOk) return kErrCuda;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return kErrArg;
-  cuuint64_t dims[2] = {(cuuint64_t)dh, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)dh};
-  cuuint32_t box[2] = {(cuuint32_t)dh, (cuuint32_t)box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        dh == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? kOk : kErrCuda;
-}
-
-inline int cuda_rc(cudaError_t e) { return e == cudaSuccess ? kOk : kErrCuda; }
-inline int launch_rc() { return cuda_rc(cudaGetLastError()); }
-
-uint32_t gbase_of(int dh) {
-  // round(2^26 / (sqrt(dh) ln 2)) with round-half-even, as Python's round() on the double
-  // (reference/lssab_golden.py:161).
-  double x = std::ldexp(1.0, kBHI) / (std::sqrt((double)dh) * std::log(2.0));
-  return (uint32_t)std::nearbyint(x);
-}
-
-inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-inline int tpad_of(int T) { return ((T + 127) / 128) * 128; }
+namespace {
 
 // ------------------------------------------------------------------ sha256 (FIPS 180-4)
 struct Sha256 {
@@ -163,34 +120,6 @@ struct Sha256 {
 const uint8_t kT2Host[kTabLive] = {
 #include "t2_table.inc"
 };
-
-// ------------------------------------------------------------------ kernel dispatch helpers
-template <typename F>
-int with_in_dtype(int dtype, F&& f) {
-  switch (dtype) {
-    case kF32: return f((const float*)nullptr);
-    case kF16: return f((const __half*)nullptr);
-    case kBF16: return f((const __nv_bfloat16*)nullptr);
-    default: return kErrArg;
-  }
-}
-
-// Launch with programmatic dependent launch: the kernel may start while the previous kernel on
-// the stream finishes; it executes griddepcontrol.wait before it reads that kernel's output.
-template <typename... KArgs, typename... Args>
-int launch_pdl(void (*kfn)(KArgs...), dim3 grid, dim3 block, int smem, cudaStream_t st, Args&&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_rc(cudaLaunchKernelEx(&cfg, kfn, std::forward<Args>(args)...));
-}
 
 template <int DH, bool SINK, typename OutT, bool GEN = false, bool KS = false>
 int launch_prefill_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PrefillArgs& a,
@@ -271,21 +200,6 @@ int launch_decode_tc_out(int out_dtype, const DecodeArgs& a, int max_splits, int
   }
 }
 
-// the vectorised quantisers need a contiguous channel dim, dh in {64, 128} and 16-byte aligned
-// rows (base and every stride a multiple of 16 bytes)
-template <typename InT>
-bool vec_ok(const void* x, const Strides4& s, int dh) {
-  const long long e = (long long)sizeof(InT);
-  return (dh == 64 || dh == 128) && s.s3 == 1 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
-         (s.s0 * e) % 16 == 0 && (s.s1 * e) % 16 == 0 && (s.s2 * e) % 16 == 0;
-}
-
-bool strides_ok(const int64_t* s, int n) {
-  if (!s) return false;
-  for (int i = 0; i < n; ++i) if (s[i] < 0) return false;
-  return true;
-}
-
 struct PrefillWs {
   size_t q8, eq, k8, ek, v8, ev, ev0, total;
 };
@@ -322,11 +236,6 @@ DecodeWs decode_ws(int B, int H, int KVH, int dh, int max_blocks) {
   w.order = o; o += align256((size_t)B * 4);                 // the refold's sequence order
   w.total = o + 256;
   return w;
-}
-
-bool shape_ok(int B, int H, int KVH, int T, int dh) {
-  return B > 0 && H > 0 && KVH > 0 && T > 0 && dh > 0 && H % KVH == 0 && dh <= 256 && dh % 32 == 0 &&
-         (long long)T <= (1ll << 24);
 }
 
 }  // namespace
@@ -433,6 +342,28 @@ static int prefill_lattice_impl(const int8_t* q8, const int32_t* eq, const int8_
               : launch_prefill_out<64, false>(out_dtype, tq, tk, tv, a, ds->num_sms, st);
 }
 
+// The decode's query quantiser ([B, H, dh] rows): the vector kernel is launched with
+// programmatic dependent launch, so it runs beside the decode plan kernel before it (which it does
+// not read); it waits for the plan before it completes, so the streaming kernel's wait on it
+// covers the plan too.  Other layouts take lssab8_quant_rows.
+int lssab8::quant_queries_pdl(const void* q, int dtype, int B, int H, int dh, const int64_t* q4, int8_t* q8,
+                              int32_t* eq, cudaStream_t st) {
+  Strides4 s{q4[0], q4[1], q4[2], q4[3]};
+  return with_in_dtype(dtype, [&](auto tag) -> int {
+    using InT = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
+    if (!vec_ok<InT>(q, s, dh)) return lssab8_quant_rows(q, dtype, B, H, 1, dh, q4, 1, q8, eq, st);
+    constexpr int N = Vec16<InT>::kN;
+    const int rpw = 32 / (dh / N);
+    const long long per_cta = 8LL * rpw * kRowsPerLane;
+    const int grid = (int)(((long long)B * H + per_cta - 1) / per_cta);
+    if (dh == 128)
+      return launch_pdl(quant_rows_vec_kernel<InT, 128>, dim3(grid), dim3(256), 0, st, static_cast<const InT*>(q), s, B,
+                        H, 1, 1, q8, eq);
+    return launch_pdl(quant_rows_vec_kernel<InT, 64>, dim3(grid), dim3(256), 0, st, static_cast<const InT*>(q), s, B, H,
+                      1, 1, q8, eq);
+  });
+}
+
 // ========================================================================== extern "C"
 extern "C" {
 
@@ -479,28 +410,6 @@ int lssab8_device_errors(int clear, void* stream, int* bits) {
     if (cudaStreamSynchronize(s) != cudaSuccess) return kErrCuda;
   }
   return kOk;
-}
-
-// The decode's query quantiser ([B, H, dh] rows): the vector kernel is launched with
-// programmatic dependent launch, so it runs beside the decode plan kernel before it (which it does
-// not read); it waits for the plan before it completes, so the streaming kernel's wait on it
-// covers the plan too.  Other layouts take lssab8_quant_rows.
-static int quant_queries_pdl(const void* q, int dtype, int B, int H, int dh, const int64_t* q4, int8_t* q8,
-                             int32_t* eq, cudaStream_t st) {
-  Strides4 s{q4[0], q4[1], q4[2], q4[3]};
-  return with_in_dtype(dtype, [&](auto tag) -> int {
-    using InT = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
-    if (!vec_ok<InT>(q, s, dh)) return lssab8_quant_rows(q, dtype, B, H, 1, dh, q4, 1, q8, eq, st);
-    constexpr int N = Vec16<InT>::kN;
-    const int rpw = 32 / (dh / N);
-    const long long per_cta = 8LL * rpw * kRowsPerLane;
-    const int grid = (int)(((long long)B * H + per_cta - 1) / per_cta);
-    if (dh == 128)
-      return launch_pdl(quant_rows_vec_kernel<InT, 128>, dim3(grid), dim3(256), 0, st, static_cast<const InT*>(q), s, B,
-                        H, 1, 1, q8, eq);
-    return launch_pdl(quant_rows_vec_kernel<InT, 64>, dim3(grid), dim3(256), 0, st, static_cast<const InT*>(q), s, B, H,
-                      1, 1, q8, eq);
-  });
 }
 
 int lssab8_quant_rows(const void* x, int dtype, int B, int H, int T, int dh, const int64_t* xs, int Tpad,
@@ -882,10 +791,11 @@ int lssab8_decode(const void* q, int dtype, const int64_t* qs, int B, int H, int
   // (the ticket reset and the plan come first so the query quantiser directly precedes the
   // decode kernel, which may then start under programmatic dependent launch)
   if (dh == 128) {                                   // the live-block plan; it also zeroes the tickets
-    decode_plan_kernel<<<1, kPlanThreads, 0, s>>>(seq_lens, B, max_blocks, max_pages,
+    decode_plan_kernel<false><<<1, kPlanThreads, 0, s>>>(seq_lens, B, max_blocks, max_pages,
                                                   reinterpret_cast<int*>(base + w.blk_off),
                                                   reinterpret_cast<int*>(base + w.order),
-                                                  reinterpret_cast<unsigned int*>(base + w.tickets), B * KVH, ds->err);
+                                                  reinterpret_cast<unsigned int*>(base + w.tickets), B * KVH, ds->err,
+                                                  0, nullptr);
     if ((rc = launch_rc())) return rc;
   } else if (cudaMemsetAsync(base + w.tickets, 0, (size_t)B * KVH * 4, s) != cudaSuccess) {
     return kErrCuda;
@@ -962,10 +872,11 @@ int lssab8_decode_noalloc(const void* q, int dtype, const int64_t* qs, int B, in
   // and the plan come first, as in lssab8_decode, so the query quantiser directly precedes the
   // decode kernel
   if (dh == 128) {                                   // the live-block plan; it also zeroes the tickets
-    decode_plan_kernel<<<1, kPlanThreads, 0, s>>>(seq_lens, B, max_blocks, max_pages,
+    decode_plan_kernel<false><<<1, kPlanThreads, 0, s>>>(seq_lens, B, max_blocks, max_pages,
                                                   reinterpret_cast<int*>(base + w.blk_off),
                                                   reinterpret_cast<int*>(base + w.order),
-                                                  reinterpret_cast<unsigned int*>(base + w.tickets), B * KVH, ds->err);
+                                                  reinterpret_cast<unsigned int*>(base + w.tickets), B * KVH, ds->err,
+                                                  0, nullptr);
     if ((rc = launch_rc())) return rc;
   } else if (cudaMemsetAsync(base + w.tickets, 0, (size_t)B * KVH * 4, s) != cudaSuccess) {
     return kErrCuda;

@@ -36,6 +36,7 @@ enum : int {
   kDevTimeout = 2,        // a bounded wait gave up (pipeline stalled)
   kDevBadPage = 4,        // block table entry out of range
   kDevAlign = 8,          // a source row off the 16-byte grid a vectorised kernel needs
+  kDevPlan = 16,          // request lengths that do not fit their buffers, or sequences that do not share a prefix
 };
 
 // dtype codes used across the C ABI
@@ -158,7 +159,7 @@ __device__ __forceinline__ float div_markstein(float y, float l, float rl) {
   const float q1 = __fmaf_rn(__fmaf_rn(-q0, l, y), rl, q0);
   return __fmaf_rn(__fmaf_rn(-q1, l, y), rl, q1);
 }
-__device__ __noinline__ float div_rn_ieee(float y, float l) { return __fdiv_rn(y, l); }
+static __device__ __noinline__ float div_rn_ieee(float y, float l) { return __fdiv_rn(y, l); }
 __device__ __forceinline__ float div_rn_shared(float y, float l, float rl) {
   if (div_window(y) && div_window(l)) return div_markstein(y, l, rl);
   return div_rn_ieee(y, l);                 // rare: kept out of line

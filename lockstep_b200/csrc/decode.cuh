@@ -44,6 +44,13 @@ struct DecodeArgs {
   void* out; long long os0, os1, os2; // out[b, h, c]
   uint32_t gbase;
   int* err;
+  // A batch that shares its first skip_blocks blocks (SHARED kernels): those blocks come from the
+  // shared-prefix kernel -- nfold folded segments, then partials -- and a block's partials are at index
+  // blk - 32 nfold of max_part.
+  int skip_blocks, nfold, max_part;
+  const int* leader;                  // the sequence whose table stands for all
+  const float* segO;                  // [B, KVH, nfold, group, dh]
+  const int2* segM;                   // [B, KVH, nfold, group] {bits of l, NB}
 };
 
 __device__ __forceinline__ uint32_t dp4a_us(uint32_t a_u8x4, uint32_t b_s8x4, uint32_t c) {
@@ -131,7 +138,9 @@ __device__ __forceinline__ void decode_merge_head(const DecodeArgs& p, int b, in
   *dst = from_f32<OutT>(y);
 }
 
-template <int DH, bool SINK, typename OutT>
+// SHARED: only the blocks after the shared ones, whose partials alone are stored (the refold is
+// decode_merge_kernel, decode_tc.cuh).
+template <int DH, bool SINK, typename OutT, bool SHARED = false>
 __global__ void __launch_bounds__(128)
 decode_kernel(const DecodeArgs p) {
   using L = DecodeSmem<DH>;
@@ -150,16 +159,20 @@ decode_kernel(const DecodeArgs p) {
   const int gq = p.group;
   const int L_len = p.seq_lens[b];
   const int nblk = (L_len + kKB - 1) / kKB;
-  const int nsplit = (nblk + p.split_blocks - 1) / p.split_blocks;
+  const int first = SHARED ? p.skip_blocks : 0;
+  const int nsplit = (nblk - first + p.split_blocks - 1) / p.split_blocks;
   if (L_len <= 0 || split >= nsplit) return;
   if (nblk > p.max_blocks || (L_len + 15) / 16 > p.max_pages) {   // lattice arrays too short
     if (tid == 0) atomicOr(p.err, kDevBadPage);
     return;
   }
-  const int blo = split * p.split_blocks;
+  const int blo = first + split * p.split_blocks;
   const int bhi = min(nblk, blo + p.split_blocks);
   const long long bg = (long long)b * p.KVH + g;
   const int32_t* bt = p.block_table + (long long)b * p.max_pages;
+  auto part_row = [&](int blk) -> long long {
+    return SHARED ? bg * p.max_part + blk - p.nfold * kSEG : bg * p.max_blocks + blk;
+  };
 
   for (int i = tid; i < kTabPad; i += blockDim.x) tab[i] = (i < kTabLive) ? kT2Live[i] : 0;
   for (int i = tid; i < gq * DH; i += blockDim.x) sq[i] = p.q8[((long long)b * p.H + g * gq) * DH + i];
@@ -285,7 +298,7 @@ decode_kernel(const DecodeArgs p) {
           }
         }
       }
-      int32_t* dstA = p.partA + ((bg * p.max_blocks + blk) * gq) * DH;
+      int32_t* dstA = p.partA + (part_row(blk) * gq) * DH;
 #pragma unroll
       for (int hh = 0; hh < 8; ++hh) if (hh < gq) dstA[hh * DH + tid] = A[hh];
     }
@@ -293,12 +306,13 @@ decode_kernel(const DecodeArgs p) {
       const int hh = tid;
       const int lb = red[32 + hh] + red[40 + hh] + red[48 + hh] + red[56 + hh];
       const int e0 = (SINK && blk == 0 && L_len > 1) ? red[64 + hh] : 0;
-      p.partM[(bg * p.max_blocks + blk) * gq + hh] = make_int4(red[72 + hh], lb, e0, 0);
+      p.partM[part_row(blk) * gq + hh] = make_int4(red[72 + hh], lb, e0, 0);
     }
     __syncthreads();                                         // stage s and red/seh are free
     if (tid == 0 && blk + 2 < bhi) issue(blk + 2, s);
   }
 
+  if (SHARED) return;
   // ---- ticket: the last split of this (sequence, kv head) merges, in ascending block order
   __threadfence();
   __syncthreads();

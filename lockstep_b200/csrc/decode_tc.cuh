@@ -72,7 +72,8 @@ constexpr int kDecChunk = 8;                       // blocks per scheduling chun
 // sequence of v is found by advancing one cursor over off (each CTA reads off once).  Sequences
 // the plan found too long for the lattice arrays have no live blocks (and are flagged there).
 // Every role runs its own copy and sees the same sequence of blocks.
-struct DecIter {
+// SHARED: the list holds the blocks after the skip_blocks shared ones only.
+template <bool SHARED> struct DecIter {
   int v, vend, chunk, nchunks, total;
   int cur_b, lo, hi, nb, L;                        // this sequence's live range [lo, hi) of v
   __device__ __forceinline__ void init(const DecodeArgs& p) {
@@ -104,7 +105,7 @@ struct DecIter {
     const int r = v++ - lo;
     b = cur_b;
     g = r / nb;
-    blk = r - g * nb;
+    blk = r - g * nb + (SHARED ? p.skip_blocks : 0);
     return true;
   }
 };
@@ -112,19 +113,23 @@ struct DecIter {
 // The live-block plan: blk_off[b] = the number of live 128-key blocks of the sequences before b
 // (blk_off[B] = all of them), one CTA, which also zeroes the refold's tickets[0 .. nticket).  A
 // sequence is live when 0 < L and its blocks and pages fit the lattice arrays; one that does not
-// fit gets no blocks and sets kDevBadPage.
+// fit gets no blocks and sets kDevBadPage.  SHARED: the first skip_blocks blocks are not counted, a
+// sequence that does not hold them sets kDevPlan, and *leader gets the first live sequence (-1: none).
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSortMax = 1024;                 // batches up to this size get the longest-first order
+template <bool SHARED>
 __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const int32_t* seq_lens, int B, int max_blocks,
                                                                     int max_pages, int* blk_off, int* order,
-                                                                    unsigned int* tickets, int nticket, int* err) {
+                                                                    unsigned int* tickets, int nticket, int* err,
+                                                                    int skip_blocks, int* leader) {
+  __shared__ int lead;
   __shared__ int warp_sums[kPlanThreads / 32];
   __shared__ int carry;
   __shared__ int sl[kPlanSortMax];
   pdl_launch_dependents();                         // the query quantiser runs beside the plan
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   for (int i = tid; i < nticket; i += kPlanThreads) tickets[i] = 0u;
-  if (tid == 0) carry = 0;
+  if (tid == 0) { carry = 0; lead = INT32_MAX; }
   __syncthreads();
   for (int base = 0; base < B; base += kPlanThreads) {
     const int i = base + tid;
@@ -135,6 +140,14 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const int32_t
       if (nb > max_blocks || (L + 15) / 16 > max_pages) {
         nb = 0;
         atomicOr(err, kDevBadPage);
+      } else if (SHARED && L > 0) {
+        nb -= skip_blocks;
+        if (L < skip_blocks * kKB) {
+          nb = 0;
+          atomicOr(err, kDevPlan);
+        } else {
+          atomicMin(&lead, i);
+        }
       }
     }
     int x = nb;                                    // inclusive warp scan
@@ -176,6 +189,7 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const int32_t
     for (int i = tid; i < B; i += kPlanThreads) order[i] = i;
   }
   if (tid == 0) blk_off[B] = carry;
+  if (SHARED && tid == 0) *leader = lead == INT32_MAX ? -1 : lead;
 }
 
 __device__ __forceinline__ uint32_t redux_max_s32(int v) {
@@ -190,7 +204,7 @@ __device__ __forceinline__ uint32_t redux_add_u32(uint32_t v) {
 }
 
 // GQ = compile-time bound on the GQA group (4: exactly 4 heads; 8: any group <= 8, masked).
-template <bool SINK, typename OutT, int GQ>
+template <bool SINK, typename OutT, int GQ, bool SHARED = false>
 __global__ void __launch_bounds__(DecWorkers<GQ>::kThreads, 2)
 decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_q,
                  const DecodeArgs p) {
@@ -241,7 +255,7 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (warp == 0) {
     // ================================================================ TMA producer
     if (lane == 0) {
-      DecIter itr;
+      DecIter<SHARED> itr;
       itr.init(p);
       int jj = 0, run = -1, cur_bg = -1, b, g, blk;
       const uint64_t once = l2_evict_first_policy();    // the lattice is read once per call
@@ -296,7 +310,7 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         umma_commit(&bars[kDPEmpty + ab]);
         return true;
       };
-      DecIter itr;
+      DecIter<SHARED> itr;
       itr.init(p);
       int jj = 0, run = -1, cur_bg = -1, b, g, blk;
       bool ok = true;
@@ -336,13 +350,16 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const int h0 = wg * GH;                              // first head of this warpgroup
     const int bar_id = 1 + wg;                           // this warpgroup's named barrier
     const uint32_t lanebase = tmem + ((uint32_t)(wq * 32) << 16);
-    DecIter itr;
+    DecIter<SHARED> itr;
     itr.init(p);
     int jj = 0, cur_bg = -1, b, g, blk;
     bool bad = false;                                    // this warp gave up a wait (decided at a barrier)
     int eqh[GH];
     // the previous block: its A partial is read out one block later, its M after the next barrier
     bool have_prev = false;
+    auto part_row = [&](long long bgx, int blkx) -> long long {
+      return SHARED ? bgx * p.max_part + blkx - p.nfold * kSEG : bgx * p.max_blocks + blkx;
+    };
     long long prev_bg = 0;
     int prev_blk = 0, prev_L = 0;
     auto readout_A = [&](int jb, long long bgx, int blkx) -> bool {
@@ -355,7 +372,7 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         tc_wait_ld();
         tc_fence_before();
         mbar_arrive(&bars[kDAEmpty + ab]);
-        int32_t* dstA = p.partA + ((bgx * p.max_blocks + blkx) * gq) * DH;
+        int32_t* dstA = p.partA + (part_row(bgx, blkx) * gq) * DH;
 #pragma unroll
         for (int hh = 0; hh < GH; ++hh) if (h0 + hh < gq) __stcg(dstA + (h0 + hh) * DH + t, (int32_t)a[hh]);
       }
@@ -366,7 +383,7 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const int h = h0 + t;
       if (t < GH && h < gq) {
         const int e0 = (SINK && blkx == 0 && Lx > 1) ? eh0s[par * 8 + h] : 0;
-        __stcg(&p.partM[(bgx * p.max_blocks + blkx) * gq + h], make_int4(nbs[par * 8 + h], (int)lbsum[par * 8 + h], e0, 0));
+        __stcg(&p.partM[part_row(bgx, blkx) * gq + h], make_int4(nbs[par * 8 + h], (int)lbsum[par * 8 + h], e0, 0));
         lbsum[par * 8 + h] = 0u;
       }
     };
@@ -478,10 +495,13 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 // and then thread t folds channels 2t and 2t + 1 with it, one exact multiply-add per block and
 // channel, while thread 32 also folds l, in the same order.  A block past the skip window gets
 // scale +0, which leaves O bit-identical (O is never -0).
+// SHARED: the first nfold segments come folded from the shared-prefix kernel, the rest of the row from
+// partials as ever; the CTA also compares its share of the sequence's first pages (and the exponents of
+// its kv head's shared blocks) with the leader's, which the shared rows were computed from: a sequence
+// that does not hold the same ones sets kDevPlan.
 constexpr int kMergeThreads = 64;
-template <bool SINK, typename OutT>
+template <bool SINK, typename OutT, int DH = 128, bool SHARED = false>
 __global__ void __launch_bounds__(kMergeThreads) decode_merge_kernel(const DecodeArgs p) {
-  constexpr int DH = 128;
   __shared__ __align__(16) int sA[kSEG][DH];
   __shared__ int2 sM[kSEG];
   __shared__ int sD[kSEG];                 // rescale distance before block u (0: none)
@@ -494,19 +514,42 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_kernel(const Decod
   const int b = p.order[blockIdx.z];
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const int c0 = 2 * t;                                // this thread's channels c0, c0 + 1
+  const bool chan = DH == 2 * kMergeThreads || c0 < DH;  // (dh 64: warp 0 alone has channels)
   const int gq = p.group;
   const int L = p.seq_lens[b];
   const int nblk = (L + kKB - 1) / kKB;
   if (L <= 0 || nblk > p.max_blocks || (L + 15) / 16 > p.max_pages) return;   // flagged by the plan
+  if (SHARED && L < p.skip_blocks * kKB) return;
+  const int max_part = SHARED ? p.max_part : p.max_blocks;
+  const int part0 = SHARED ? p.nfold * kSEG : 0;       // the first block that has partials
   const long long bg = (long long)b * p.KVH + g;
-  const int4* pm = p.partM + (bg * p.max_blocks) * gq + h;      // block u's {NB, l_b, eh0} at pm[u * gq]
+  const int4* pm = p.partM + (bg * max_part - part0) * gq + h;  // block u's {NB, l_b, eh0} at pm[u * gq]
   const int32_t* evb = p.ev + bg * p.max_blocks;
   int v0a = 0, v0b = 0, evs0 = 0, eh0 = 0;
-  if (SINK && L > 1) {
-    const int pg = p.block_table[(long long)b * p.max_pages];
+  if (SHARED) {
+    const int ld = p.leader[0];
+    if (b != ld) {
+      const int32_t* mine = p.block_table + (long long)b * p.max_pages;
+      const int32_t* lead = p.block_table + (long long)ld * p.max_pages;
+      bool same = true;
+      for (int i = (g * gq + h) * kMergeThreads + t; i < p.skip_blocks * 8; i += p.H * kMergeThreads)
+        same = same && mine[i] == lead[i];
+      const long long lg = (long long)ld * p.KVH + g;
+      for (int i = h * kMergeThreads + t; i < p.skip_blocks; i += gq * kMergeThreads)
+        same = same && p.ek[bg * p.max_blocks + i] == p.ek[lg * p.max_blocks + i] &&
+               p.ev[bg * p.max_blocks + i] == p.ev[lg * p.max_blocks + i];
+      if (SINK && h == 0 && t == 0) same = same && p.ev0[bg] == p.ev0[lg];
+      if (!same) atomicOr(p.err, kDevPlan);
+    }
+  }
+  if (SINK && L > 1 && part0 == 0) {
+    int pg = p.block_table[(long long)b * p.max_pages];
+    if (SHARED && (pg < 0 || pg >= p.num_pages)) pg = 0;       // flagged where its page was loaded
     const int8_t* v0 = p.v8p + ((long long)pg * p.KVH + g) * (16 * DH);
-    v0a = (int)v0[c0 * 16];
-    v0b = (int)v0[(c0 + 1) * 16];
+    if (chan) {
+      v0a = (int)v0[c0 * 16];
+      v0b = (int)v0[(c0 + 1) * 16];
+    }
     evs0 = p.ev0[bg];
     eh0 = __ldcg(&pm[0]).z;
   }
@@ -514,15 +557,35 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_kernel(const Decod
   int nbrow = 0;                                       // thread 0 only
   int2 mn = make_int2(INT32_MIN, 0);                   // warp 0: the segment's schedule inputs, one block per lane
   int evn = 0;
-  if (w == 0 && lane < min(kSEG, nblk)) {
-    mn = __ldcg(reinterpret_cast<const int2*>(&pm[lane * gq]));
-    evn = evb[lane];
+  if (w == 0 && lane < min(kSEG, nblk - part0)) {
+    mn = __ldcg(reinterpret_cast<const int2*>(&pm[(part0 + lane) * gq]));
+    evn = evb[part0 + lane];
   }
-  for (int s0 = 0; s0 < nblk; s0 += kSEG) {
+  if (SHARED) {                                        // the folded segments -> row, the same rules as below
+    const int2* sm = p.segM + bg * p.nfold * gq + h;
+    const float* so = p.segO + (bg * p.nfold * gq + h) * DH + c0;
+#pragma unroll 4
+    for (int s = 0; s < p.nfold; ++s) {
+      const int2 m = __ldcg(sm + (long long)s * gq);
+      const float2 x = chan ? __ldcg(reinterpret_cast<const float2*>(so + (long long)s * gq * DH)) : make_float2(0.0f, 0.0f);
+      if (s == 0) nbrow = m.y;
+      const int d = m.y - nbrow;
+      if (d > 0) { Oa = rescale(Oa, d); Ob = rescale(Ob, d); lrow = rescale(lrow, d); nbrow = m.y; }
+      const int s2 = d > 0 ? 0 : -d;
+      if (s2 <= kSWIN) {
+        Oa = __fadd_rn(Oa, rescale(x.x, s2));
+        Ob = __fadd_rn(Ob, rescale(x.y, s2));
+        lrow = __fadd_rn(lrow, rescale(__int_as_float(m.x), s2));
+      }
+    }
+    if (t == 32) sLrow = lrow;                         // (a row may end with its last folded segment)
+    __syncthreads();
+  }
+  for (int s0 = part0; s0 < nblk; s0 += kSEG) {
     const int n = min(kSEG, nblk - s0);
     for (int i = t; i < n * (DH / 4); i += kMergeThreads) {     // 16-byte pieces of the n partial rows
       const int u = i / (DH / 4), q = i % (DH / 4);
-      const int32_t* src = p.partA + ((bg * p.max_blocks + s0 + u) * gq + h) * DH + q * 4;
+      const int32_t* src = p.partA + ((bg * max_part - part0 + s0 + u) * gq + h) * DH + q * 4;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&sA[u][q * 4])), "l"(src) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -576,7 +639,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_kernel(const Decod
         xa = fold_term(xa, eh0 * v0a, sc0);
         xb = fold_term(xb, eh0 * v0b, sc0);
       }
-      const int2 av = *reinterpret_cast<const int2*>(&sA[u][c0]);
+      const int2 av = chan ? *reinterpret_cast<const int2*>(&sA[u][c0]) : make_int2(0, 0);
       const float sc = sSc[u];
       xa = fold_term(xa, av.x, sc);
       xb = fold_term(xb, av.y, sc);
@@ -598,6 +661,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_kernel(const Decod
   }
   const float lr = sLrow;
   OutT* dst = reinterpret_cast<OutT*>(p.out) + b * p.os0 + (long long)(g * gq + h) * p.os1 + c0 * p.os2;
+  if (!chan) return;
   dst[0] = from_f32<OutT>(lr != 0.0f ? __fdiv_rn(Oa, lr) : 0.0f);
   dst[p.os2] = from_f32<OutT>(lr != 0.0f ? __fdiv_rn(Ob, lr) : 0.0f);
 }

@@ -59,10 +59,42 @@
 // (reference/lssab8_torch.py:203-271, reference/lssab8_golden.py:257-335).  B9.1 sink_alone
 // (reference/lssab9_torch.py:276-304): key 0's weight is removed from block 0's P operand
 // (l_b keeps it) and its product eh0 * v8[0] is folded first with e_v0.
+// The paged forms (SRC; paged.cuh plans and launches them) run the same roles over the decode's paged
+// lattice: a block is 8 key pages (boxes of 16 rows, swizzled like a 128-row box) and 8 value pages as
+// they are, [channel][16 keys] -- 8-channel x 16-key core matrices, the K-major B operand of the PV MMA.
+//   kSrcRows    packed prompt rows: items are (128-row tile of one sequence, head); a row sees the keys of
+//               its own sequence up to itself, or up to its sequence's bidirectional prefix if that is
+//               farther (every row of a tile sees a key of every block the tile walks).
+//   kSrcShared  rows are the (sequence, head) pairs of one kv head, 128 / group sequences a tile, against
+//               blocks of the prefix they share.  A row's fold is sequential, so an item is either a whole
+//               32-block segment, folded in TMEM and stored as (O, l, NB), or a few blocks whose exact
+//               partials are stored for the refold, as the decode's are.
 #pragma once
 #include "tcgen05.cuh"
 
 namespace lssab8 {
+enum : int { kSrcDense = 0, kSrcRows = 1, kSrcShared = 2 };
+// The paged forms' arguments.
+struct PagedArgs {
+  int max_blocks, max_pages, num_pages;
+  const int32_t* block_table;   // [B, max_pages]
+  const int32_t* seq_lens;      // [B]
+  const int8_t* v8p;            // [P, KVH, dh, 16]
+  // kSrcRows
+  const int4* tiles;            // {sequence, diagonal block, blocks, first row of q}, longest first
+  const int* ntiles;
+  const int32_t* prefix;        // [B] or nullptr
+  // kSrcShared
+  const int* leader;            // the sequence whose table and exponents stand for all (-1: none is live)
+  int seqs_per_tile, row_tiles; // sequences of a 128-row tile; tiles of the batch
+  int nfold, chunk, nchunks;    // folded segments, then nchunks items of chunk blocks a (tile, kv head)
+  int shared_blocks;
+  int max_part;                 // partials of block blk at index blk - 32 nfold of max_part
+  int32_t* partA;               // [B, KVH, max_part, group, dh]
+  int4* partM;                  // [B, KVH, max_part, group]
+  float* segO;                  // [B, KVH, nfold, group, dh]
+  int2* segM;                   // [B, KVH, nfold, group] {bits of l, NB}
+};
 constexpr int kMaxPeers = 7;                                  // other ranks of one 8-GPU node
 struct PrefillArgs {
   int B, H, KVH, T, dh, Tpad, nblk, group;
@@ -93,6 +125,7 @@ struct PrefillArgs {
   int causal;
   const uint32_t* kmask;
   const int8_t* d8;     // B9.3 (KS kernels): per-key weight shift [B, KVH, nblk * 128]
+  PagedArgs pg;         // the paged forms (SRC kernels)
 };
 
 // ------------------------------------------------------------------------ smem layout
@@ -128,6 +161,10 @@ enum BarId : int {
 struct PfItem {
   int tile, b, h;
   int kt;               // the tile's key-block index: tile0 + tile (the diagonal block)
+  // the paged forms
+  int g, T, nb, j0;     // kv head, the sequence's length, blocks of the item, its first block
+  int row0, prefix;     // kSrcRows: first row of q; bidirectional prefix
+  bool fold;            // kSrcShared: a whole segment
 };
 __device__ __forceinline__ bool pf_item(const PrefillArgs& p, int ntile, int round, PfItem& it) {
   const int G = gridDim.x;
@@ -138,6 +175,38 @@ __device__ __forceinline__ bool pf_item(const PrefillArgs& p, int ntile, int rou
   it.kt = p.tile0 + it.tile;
   it.b = bh / p.H;
   it.h = bh % p.H;
+  return true;
+}
+// Items of the paged forms, the same snake order.
+template <int SRC> __device__ __forceinline__ int pf_paged_items(const PrefillArgs& p) {
+  if constexpr (SRC == kSrcRows) return p.pg.ntiles[0] * p.H;
+  return p.pg.leader[0] < 0 ? 0 : p.KVH * p.pg.row_tiles * (p.pg.nfold + p.pg.nchunks);
+}
+template <int SRC>
+__device__ __forceinline__ bool pf_item_paged(const PrefillArgs& p, int total, int round, PfItem& it) {
+  const int G = gridDim.x;
+  const int i = round * G + ((round & 1) ? (G - 1 - (int)blockIdx.x) : (int)blockIdx.x);
+  if (i >= total) return false;
+  if constexpr (SRC == kSrcRows) {
+    const int4 t = p.pg.tiles[i / p.H];
+    it.h = i % p.H;
+    it.g = it.h / p.group;
+    it.b = t.x;
+    it.kt = t.y;
+    it.nb = t.z;
+    it.row0 = t.w;
+    it.j0 = 0;
+    it.prefix = p.pg.prefix ? p.pg.prefix[it.b] : 0;
+  } else {
+    const int gt = i % (p.KVH * p.pg.row_tiles), c = i / (p.KVH * p.pg.row_tiles);
+    it.g = gt / p.pg.row_tiles;              // a block's row tiles run side by side: its pages come from L2
+    it.tile = gt % p.pg.row_tiles;
+    it.b = p.pg.leader[0];
+    it.fold = c < p.pg.nfold;
+    it.j0 = it.fold ? c * kSEG : p.pg.nfold * kSEG + (c - p.pg.nfold) * p.pg.chunk;
+    it.nb = it.fold ? kSEG : min(p.pg.chunk, p.pg.shared_blocks - it.j0);
+  }
+  it.T = p.pg.seq_lens[it.b];
   return true;
 }
 // TMEM column map: S, A (two buffers of 128; one in the MULTI kernel), O_row (MULTI), O (O_seg)
@@ -215,7 +284,7 @@ __device__ __forceinline__ void store_chunk(OutT* dst, long long os3, const floa
   }
 }
 
-template <int DH, bool SINK, typename OutT, bool MULTI, bool GEN = false, bool KS = false>
+template <int DH, bool SINK, typename OutT, bool MULTI, bool GEN = false, bool KS = false, int SRC = kSrcDense>
 __global__ void __launch_bounds__(kPrefillThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const PrefillArgs p) {
@@ -233,8 +302,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   int8_t* v0row = reinterpret_cast<int8_t*>(smem + L::kV0);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr bool PAGED = SRC != kSrcDense;
   const int ntile = p.Tpad / 128;
-  const int nrounds = (ntile * p.B * p.H + (int)gridDim.x - 1) / (int)gridDim.x;
+  int nrounds = PAGED ? 0 : (ntile * p.B * p.H + (int)gridDim.x - 1) / (int)gridDim.x;
+  int nitems = 0;                                    // paged: known once the plan has run
+  auto next_item = [&](int rd, PfItem& it) -> bool {
+    if constexpr (PAGED) return pf_item_paged<SRC>(p, nitems, rd, it);
+    else return pf_item(p, ntile, rd, it);
+  };
 
   // ---- setup, once per CTA: barriers, T2 copies, TMEM
   if (threadIdx.x == 0) {
@@ -284,6 +359,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   pdl_wait();                                        // the quantisers' lattice is complete
+  if constexpr (PAGED) {
+    nitems = pf_paged_items<SRC>(p);
+    nrounds = (nitems + (int)gridDim.x - 1) / (int)gridDim.x;
+  }
 
   if (warp == 0) {
     // ================================================================ TMA producer
@@ -292,13 +371,53 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       bool ok = true;
       PfItem it;
       for (int rd = 0; ok && rd < nrounds; ++rd) {
-        if (!pf_item(p, ntile, rd, it)) continue;
+        if (!next_item(rd, it)) continue;
         const int g = it.h / p.group;
         const int qrow0 = (it.b * p.H + it.h) * p.Tpad + it.tile * 128;
         const int krow0 = (it.b * p.KVH + g) * (p.nblk * 128);
         const int qb = tt & 1;
         // buffer qb is free once item tt - 2's last QK has finished and its workers are done
         if (!mbar_wait(&bars[kBarQEmpty + qb], ((tt >> 1) & 1) ^ 1, abort_flag, p.err, 128, p.wait_ns)) { ok = false; break; }
+        if constexpr (PAGED) {
+          constexpr uint32_t kPage = 16 * DH;
+          if constexpr (SRC == kSrcRows) {
+            mbar_expect_tx(&bars[kBarQFull + qb], L::kTile);
+            tma_load_2d(smem + L::kQ + qb * L::kTile, &tm_q, 0, it.h * p.Tpad + it.row0, &bars[kBarQFull + qb]);
+          } else {
+            mbar_expect_tx(&bars[kBarQFull + qb], (uint32_t)(p.pg.seqs_per_tile * p.group * DH));
+            tma_load_3d(smem + L::kQ + qb * L::kTile, &tm_q, 0, it.g * p.group, it.tile * p.pg.seqs_per_tile,
+                        &bars[kBarQFull + qb]);
+          }
+          const int32_t* bt = p.pg.block_table + (long long)it.b * p.pg.max_pages;
+          const int npages = (it.T + 15) / 16;
+          for (int j = 0; j < it.nb; ++j, ++jj) {
+            const int s = jj & 1;
+            const uint32_t ph = (jj >> 1) & 1;
+            const int p0 = (it.j0 + j) * 8;
+            const int npg = min(8, npages - p0);
+            long long pr[8];                             // page rows, in flight during the wait
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pr[i] = i < npg ? bt[p0 + i] : 0;
+            if (!mbar_wait(&bars[kBarKEmpty + s], ph ^ 1, abort_flag, p.err, 128, p.wait_ns)) { ok = false; break; }
+            mbar_expect_tx(&bars[kBarKFull + s], npg * kPage);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (i >= npg) break;
+              if (pr[i] < 0 || pr[i] >= p.pg.num_pages) { atomicOr(p.err, kDevBadPage); pr[i] = 0; }
+              pr[i] = pr[i] * p.KVH + it.g;
+              tma_load_2d(smem + L::kK + s * L::kTile + i * kPage, &tm_k, 0, (int)(pr[i] * 16), &bars[kBarKFull + s]);
+            }
+            if (!mbar_wait(&bars[kBarVEmpty + s], ph ^ 1, abort_flag, p.err, 128, p.wait_ns)) { ok = false; break; }
+            mbar_expect_tx(&bars[kBarVFull + s], npg * kPage);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (i >= npg) break;
+              bulk_g2s(smem + L::kV + s * L::kTile + i * kPage, p.pg.v8p + pr[i] * kPage, kPage, &bars[kBarVFull + s]);
+            }
+          }
+          ++tt;
+          continue;
+        }
         mbar_expect_tx(&bars[kBarQFull + qb], L::kTile + (SINK ? DH : 0));
         tma_load_2d(smem + L::kQ + qb * L::kTile, &tm_q, 0, qrow0, &bars[kBarQFull + qb]);
         if (SINK) bulk_g2s(v0row + qb * 128, p.v8 + (long long)krow0 * DH, DH, &bars[kBarQFull + qb]);
@@ -324,7 +443,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       constexpr uint32_t kSwz = (DH == 128) ? 2u : 4u;          // 128B / 64B swizzle
       constexpr uint32_t kRowGroup = 8 * DH;                    // bytes per 8 rows of a tile
       constexpr uint32_t idesc_qk = idesc_i8(1, 1, 0, 128, 128);
-      constexpr uint32_t idesc_pv = idesc_i8(0, 1, 1, 128, DH);
+      constexpr uint32_t idesc_pv = idesc_i8(0, 1, PAGED ? 0 : 1, 128, DH);
       // the bias block as a no-swizzle 128-row x 32-byte matrix: core matrices of 8 rows x 16 B,
       // 128 B apart along a row, 256 B apart down the rows (every word is the same, so only the
       // extent matters: the copy reads 4 KB)
@@ -351,8 +470,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       };
       PfItem it;
       for (int rd = 0; ok && rd < nrounds; ++rd) {
-        if (!pf_item(p, ntile, rd, it)) continue;
-        const int nb = (GEN && !p.causal) ? p.nblk : it.kt + 1;
+        if (!next_item(rd, it)) continue;
+        const int nb = PAGED ? it.nb : (GEN && !p.causal) ? p.nblk : it.kt + 1;
         const int qb = tt & 1;
         if (!mbar_wait(&bars[kBarQFull + qb], (tt >> 1) & 1, abort_flag, p.err, 0, p.wait_ns)) { ok = false; break; }
         const uint32_t sq = smem_u32(smem + L::kQ + qb * L::kTile);
@@ -382,8 +501,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             // A = P (K-major SW128, 32 keys = 32 bytes per step); B = V (MN-major: 32 keys =
             // 4 groups of 8 rows per step; LBO = MN-atom stride (one atom), SBO = 8-row stride).
             // Every step accumulates: the accumulator starts at the 1.5 * 2^23 bias.
+            // Value pages (paged) are K-major core matrices: LBO = one page (16 keys), SBO = 8 channels.
             umma_i8(tmem + kColA + sa * 128, umma_desc(sp + kk * 32, 16, 1024, 2),
-                    umma_desc(sv + kk * 32 * DH, L::kTile, kRowGroup, kSwz), idesc_pv, 1u);
+                    PAGED ? umma_desc(sv + kk * 32 * DH, 16 * DH, 128, 0)
+                          : umma_desc(sv + kk * 32 * DH, L::kTile, kRowGroup, kSwz), idesc_pv, 1u);
           }
           umma_commit(&bars[kBarAFull + sa]);
           umma_commit(&bars[kBarVEmpty + s]);
@@ -418,17 +539,41 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     bool ok = true;
     PfItem it;
     for (int rd = 0; ok && rd < nrounds; ++rd) {
-      if (!pf_item(p, ntile, rd, it)) continue;
+      if (!next_item(rd, it)) continue;
       const int tile = it.tile, kt = it.kt, b = it.b, h = it.h;
-      const int g = h / p.group;
-      const int nb = (GEN && !p.causal) ? p.nblk : kt + 1;   // causal: key blocks 0 .. kt
-      const int qrow0 = (b * p.H + h) * p.Tpad + tile * 128;
+      const int g = PAGED ? it.g : h / p.group;
+      const int nb = PAGED ? it.nb : (GEN && !p.causal) ? p.nblk : kt + 1;   // causal: key blocks 0 .. kt
       const int qb = tt & 1;
-      const int8_t* v0 = v0row + qb * 128;               // key 0's value row of this item (sink)
-      const int eqr = p.eq[(long long)qrow0 + r];
-      const int32_t* ekg = p.ek + (long long)(b * p.KVH + g) * p.nblk;
-      const int32_t* evg = p.ev + (long long)(b * p.KVH + g) * p.nblk;
+      const int T = PAGED ? it.T : p.T;
+      const bool sink0 = SINK && T > 1 && (!PAGED || it.j0 == 0);   // block 0 of this item holds key 0's own term
+      // key 0's value row (sink): the item's staged copy, or its channels in the first value page
+      const int8_t* v0 = v0row + qb * 128;
+      int eqr, srow = 0;                                 // srow (kSrcShared): this row's (sequence, head) pair, or -1
+      const int32_t *ekg, *evg;
+      if constexpr (PAGED) {
+        if constexpr (SRC == kSrcRows) {
+          eqr = p.eq[(long long)h * p.Tpad + it.row0 + r];
+        } else {
+          const int sq = r / p.group, seq = tile * p.pg.seqs_per_tile + sq;
+          srow = (sq < p.pg.seqs_per_tile && seq < p.B) ? seq * p.H + g * p.group + (r - sq * p.group) : -1;
+          eqr = srow >= 0 ? p.eq[srow] : 0;
+        }
+        ekg = p.ek + ((long long)b * p.KVH + g) * p.pg.max_blocks + it.j0;
+        evg = p.ev + ((long long)b * p.KVH + g) * p.pg.max_blocks + it.j0;
+        if (SINK) {
+          const int pg0 = p.pg.block_table[(long long)b * p.pg.max_pages];
+          v0 = p.pg.v8p + ((long long)((pg0 < 0 || pg0 >= p.pg.num_pages) ? 0 : pg0) * p.KVH + g) * (16 * DH);
+        }
+      } else {
+        const int qrow0 = (b * p.H + h) * p.Tpad + tile * 128;
+        eqr = p.eq[(long long)qrow0 + r];
+        ekg = p.ek + (long long)(b * p.KVH + g) * p.nblk;
+        evg = p.ev + (long long)(b * p.KVH + g) * p.nblk;
+      }
+      constexpr int kV0Step = PAGED ? 16 : 1;
       const int ev0 = SINK ? p.ev0[b * p.KVH + g] : 0;
+      // kSrcRows: the last position this row sees
+      const int last = SRC == kSrcRows ? max(kt * 128 + r, it.prefix - 1) : 0;
       // fold state: both lanes of a row compute it identically
       float lseg = 0.0f, lrow = 0.0f;
       int nbrun = 0, nbrow = 0;
@@ -453,7 +598,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         }
         if (!warp_poll(&bars[kBarAFull + sa], pha, abort_flag, p.err, p.wait_ns)) return false;
         // key 0's value row arrives with the item's Q tile
-        if (SINK && jf == 0 && p.T > 1 && !warp_poll(&bars[kBarQFull + qb], (tt >> 1) & 1, abort_flag, p.err, p.wait_ns)) return false;
+        if (!PAGED && sink0 && jf == 0 && !warp_poll(&bars[kBarQFull + qb], (tt >> 1) & 1, abort_flag, p.err, p.wait_ns)) return false;
         tc_fence_after();
         // A block beyond the exact-skip window (sg > S_WIN) is folded with scale +0 instead of being
         // skipped: O and l are never -0 (they start at +0, an RN sum that cancels exactly is +0, and
@@ -472,13 +617,13 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const uint32_t abase = rowt + kColA + sa * 128;
         auto fold_pass = [&](int c0, uint32_t* a, uint32_t* o) {
           if (resc) rescale_channels<kPass>(o, Dr, sD2);
-          if (SINK && jf == 0 && p.T > 1) {                  // key 0's term first (B9.1); sg == 0 here
+          if (SINK && sink0 && jf == 0) {                    // key 0's term first (B9.1); sg == 0 here
             const float sc0 = pow2f(-ev0);
             const uint64_t sc02 = f2_pack(sc0, sc0);
   #pragma unroll
             for (int t = 0; t < kPass / 2; ++t) {
               const int c = kh * HALF + c0 + 2 * t;
-              const uint64_t z = f2_pack(i2f_small(eh0v * (int)v0[c]), i2f_small(eh0v * (int)v0[c + 1]));
+              const uint64_t z = f2_pack(i2f_small(eh0v * (int)v0[c * kV0Step]), i2f_small(eh0v * (int)v0[(c + 1) * kV0Step]));
               float lo_, hi_;
               f2_unpack(f2_fma(z, sc02, f2_pack(__uint_as_float(o[2 * t]), __uint_as_float(o[2 * t + 1]))), lo_, hi_);
               o[2 * t] = __float_as_uint(lo_);
@@ -568,6 +713,39 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         return true;
       };
 
+      // kSrcShared, an item of a few blocks: the exact partials of block jf, as the decode stores them
+      auto store_partials = [&](int jf, int nbb, int lbt, int eh0v) -> bool {
+        const int jgf = jj0 + jf;
+        const int sa = jgf & 1;
+        if (!warp_poll(&bars[kBarAFull + sa], (uint32_t)((jgf >> 1) & 1), abort_flag, p.err, p.wait_ns)) return false;
+        tc_fence_after();
+        const uint32_t abase = rowt + kColA + sa * 128;
+        const int seq = srow / p.H, hh = srow - seq * p.H - g * p.group;
+        const long long row = (((long long)seq * p.KVH + g) * p.pg.max_part + it.j0 + jf - p.pg.nfold * kSEG) * p.group + hh;
+  #pragma unroll
+        for (int cc = 0; cc < HALF / 16; ++cc) {
+          uint32_t a[16];
+          tmem_ld16x2<HALF>(abase + cc * 16, a);
+          tc_wait_ld();
+          if (srow >= 0) {
+            int4* dst = reinterpret_cast<int4*>(p.pg.partA + row * DH + kh * HALF + cc * 16);
+  #pragma unroll
+            for (int c = 0; c < 4; ++c)
+              __stcg(dst + c, make_int4((int)(a[4 * c] - kMagicBits), (int)(a[4 * c + 1] - kMagicBits),
+                                        (int)(a[4 * c + 2] - kMagicBits), (int)(a[4 * c + 3] - kMagicBits)));
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&bars[kBarAEmpty + sa]);
+        if (srow >= 0 && kh == 0) __stcg(p.pg.partM + row, make_int4(nbb, lbt, sink0 && jf == 0 ? eh0v : 0, 0));
+        return true;
+      };
+      auto finish_block = [&](int jf, int nbb, int lbt, int evj, int eh0v, bool live) -> bool {
+        if constexpr (SRC == kSrcShared) {
+          if (!it.fold) return store_partials(jf, nbb, lbt, eh0v);
+        }
+        return fold_block(jf, nbb, lbt, evj, eh0v, live);
+      };
       int nb_prev = 0, ev_prev = 0, lbt_prev = 0, eh0_row = 0;
       bool live_prev = true;
       int ek_next = ekg[0], ev_next = evg[0];            // e_k, e_v one block ahead
@@ -609,7 +787,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         if (!warp_poll(&bars[kBarPEmpty + s], ph ^ 1, abort_flag, p.err, p.wait_ns)) { ok = false; break; }
         if (!warp_poll(&bars[kBarSFull], jg & 1, abort_flag, p.err, p.wait_ns)) { ok = false; break; }
         tc_fence_after();
-        const bool diag = (j == kt) && (!GEN || p.causal);  // key c of the diagonal block visible iff c <= r
+        const bool diag = !PAGED && (j == kt) && (!GEN || p.causal);  // key c of the diagonal block visible iff c <= r
         // pass 1: this lane's 64 scores into registers (one TMEM round trip; S is free for the
         // next QK as soon as they have landed) and the exact max over its visible keys
         uint32_t v[64];
@@ -624,6 +802,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         if (diag) {
   #pragma unroll
           for (int c = 0; c < 64; ++c) if (kh * 64 + c > r) v[c] = 0x80000000u;
+        }
+        if (SRC == kSrcRows && j >= kt) {                  // keys past the last one this row sees
+          const int end = last - j * 128 - kh * 64;
+  #pragma unroll
+          for (int c = 0; c < 64; ++c) if (c > end) v[c] = 0x80000000u;
         }
         if (GEN) {                                         // hidden keys
   #pragma unroll
@@ -676,7 +859,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             }
           }
           const int chunk = kh * 4 + cc;
-          if (SINK && chunk == 0 && j == 0 && p.T > 1) { eh0 = w[0] & 0xFFu; w[0] &= ~0xFFu; }
+          if (SINK && chunk == 0 && j == 0 && sink0) { eh0 = w[0] & 0xFFu; w[0] &= ~0xFFu; }
           st_shared_v4(pbase + (uint32_t)((chunk ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
         }
         fence_async_smem();
@@ -684,26 +867,46 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const uint32_t lb = lbq[0] + lbq[1];
         const int lbt = (int)lb + __shfl_xor_sync(0xffffffffu, (int)lb, 16);   // the row's l_b
         if (SINK && j == 0) eh0_row = __shfl_sync(0xffffffffu, (int)eh0, lane & 15);
-        if (j > 0 && !fold_block(j - 1, nb_prev, lbt_prev, ev_prev, eh0_row, live_prev)) { ok = false; break; }
+        if (j > 0 && !finish_block(j - 1, nb_prev, lbt_prev, ev_prev, eh0_row, live_prev)) { ok = false; break; }
         nb_prev = nbv;
         lbt_prev = lbt;
         ev_prev = evj;
         live_prev = live;
       }
-      if (ok) ok = fold_block(nb - 1, nb_prev, lbt_prev, ev_prev, eh0_row, live_prev);
+      if (ok) ok = finish_block(nb - 1, nb_prev, lbt_prev, ev_prev, eh0_row, live_prev);
 
       // ---- epilogue: out = O_row / l_row (one RN division per element; l_row == 0 -> 0).
       // `ok` is warp-uniform (every wait is decided for the whole warp), so the warp-collective
       // TMEM loads run on every lane or on none; rows past T skip only the store.
-      if (ok) {
+      if constexpr (SRC == kSrcShared) {                 // a folded segment's state, as it is
+        if (ok && it.fold) {
+          const int seq = srow / p.H, hh = srow - seq * p.H - g * p.group;
+          const long long row = (((long long)seq * p.KVH + g) * p.pg.nfold + it.j0 / kSEG) * p.group + hh;
+  #pragma unroll 1
+          for (int cc = 0; cc < HALF / 16; ++cc) {
+            uint32_t y[16];
+            tmem_ld16x2<HALF>(obase + cc * 16, y);
+            tc_wait_ld();
+            tmem_fill16x2<HALF>(obase + cc * 16, 0u);
+            if (srow >= 0) {
+              uint4* dst = reinterpret_cast<uint4*>(p.pg.segO + row * DH + kh * HALF + cc * 16);
+  #pragma unroll
+              for (int c = 0; c < 4; ++c) __stcg(dst + c, make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]));
+            }
+          }
+          tc_wait_st();
+          if (srow >= 0 && kh == 0) __stcg(p.pg.segM + row, make_int2(__float_as_int(lseg), nbrun));
+        }
+      } else if (ok) {
         if (!mseg) lrow = rescale(lseg, 0);             // a single segment: O_row = 0 + rescale(O_seg, 0)
         const int i = kt * 128 + r;                      // the row's position in the sequence
-        const bool live = (i < p.T);
+        const bool live = (i < T);
         const bool nz = (lrow != 0.0f);
         const float rl = nz ? __frcp_rn(lrow) : 0.0f;
         const bool row_fast = div_window(lrow);
-        OutT* dst = reinterpret_cast<OutT*>(p.out) + b * p.os0 + (long long)(i - p.tile0 * 128) * p.os1 + h * p.os2 +
-                    kh * HALF * p.os3;                   // out holds the chunk's rows
+        OutT* dst = reinterpret_cast<OutT*>(p.out) + (PAGED ? 0 : b * p.os0) +
+                    (long long)(PAGED ? it.row0 + r : i - p.tile0 * 128) * p.os1 + h * p.os2 +
+                    kh * HALF * p.os3;                   // out holds the chunk's (the packed) rows
   #pragma unroll 1
         for (int cc = 0; cc < HALF / 16; ++cc) {
           float q[16];

@@ -210,3 +210,111 @@ def decode(q, kv, split_blocks=4, out=None, out_dtype=None, check=True):
     if check:
         _A.check_device_errors(dev)
     return out
+
+
+def _check_lattice(q, kv, B, H, dh):
+    dev = _A._require_cuda(q, kv.k8p, kv.seq_lens, kv.block_table, kv.ek, kv.ev)
+    if dh != kv.dh or kv.seq_lens.numel() != B or kv.block_table.shape[0] != B or H % kv.KVH:
+        raise ValueError("query does not match the lattice")
+    if not (kv.seq_lens.is_contiguous() and kv.block_table.is_contiguous() and kv.ek.is_contiguous() and
+            kv.ev.is_contiguous() and kv.ev0.is_contiguous()):
+        raise ValueError("the lattice's lengths, table and exponents must be contiguous")
+    if kv.seq_lens.dtype != torch.int32 or kv.block_table.dtype != torch.int32:
+        raise TypeError("the lattice's lengths and table must be int32")
+    return dev
+
+
+def _check_out(out, shape, dev):
+    if tuple(out.shape) != tuple(shape) or out.device != dev:
+        raise ValueError("out must be %s on the query's device" % (tuple(shape),))
+
+
+def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtype=None, check=True):
+    """All prompt rows of a step in one call, over the paged lattice that already holds their keys (append_kv
+    or build_paged_kv first): q [N, H, dh] -> out [N, H, dh] (default q.dtype).
+
+    Sequence b's rows are q[cu_q[b]:cu_q[b + 1]] (cu_q [B + 1] int32, CUDA) and stand at its last positions,
+    [T0, kv.seq_lens[b]) with T0 a multiple of 128.  Each row sees only its own sequence's keys (document
+    mask): up to its own position, or up to the sequence's bidirectional prefix prefix_lens[b] (int32 [B]) if
+    that is farther (prefix mask).  Without a prefix every row is bit-identical to the prefill of its sequence
+    alone.  active [B] bool: the sequences that have rows here (None: all); other rows of out, and rows outside
+    cu_q, stay as they were (a new out: undefined).  Lengths that break these rules raise RuntimeError
+    (device error 16) when checked."""
+    if q.dim() != 3:
+        raise ValueError("q must be [N, H, dh]")
+    N, H, dh = q.shape
+    B = kv.seq_lens.numel()
+    dev = _check_lattice(q, kv, B, H, dh)
+    _A._require_cuda(q, cu_q, *[t for t in (prefix_lens, active) if t is not None])
+    if tuple(cu_q.shape) != (B + 1,) or cu_q.dtype != torch.int32:
+        raise ValueError("cu_q must be [%d] int32" % (B + 1))
+    if prefix_lens is not None and (tuple(prefix_lens.shape) != (B,) or prefix_lens.dtype != torch.int32):
+        raise ValueError("prefix_lens must be [%d] int32" % B)
+    if active is not None and (tuple(active.shape) != (B,) or active.dtype != torch.bool):
+        raise ValueError("active must be [%d] bool" % B)
+    if out is None:
+        out = torch.empty((N, H, dh), dtype=out_dtype or q.dtype, device=dev)
+    _check_out(out, (N, H, dh), dev)
+    if N == 0:
+        return out
+    cu_q = cu_q.contiguous()
+    prefix_lens = None if prefix_lens is None else prefix_lens.contiguous()
+    active = None if active is None else active.contiguous()
+    L = _lib.load()
+    nbytes = L.lssab8_prefill_paged_workspace_size(N, H, kv.KVH, dh, B)
+    if nbytes == 0:
+        raise ValueError("unsupported shape")
+    # the workspace comes from torch's allocator on this stream at every call, so calls on other streams
+    # and captured graphs never share one
+    with torch.cuda.device(dev):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.check(L.lssab8_prefill_paged(
+            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64x(q.stride()), N, H, kv.KVH, dh, cu_q.data_ptr(),
+            kv.seq_lens.data_ptr(), None if prefix_lens is None else prefix_lens.data_ptr(),
+            None if active is None else active.data_ptr(), B, kv.block_table.data_ptr(), kv.block_table.shape[1],
+            kv.num_pages, kv.k8p.data_ptr(), kv.v8p.data_ptr(), kv.ek.data_ptr(), kv.ev.data_ptr(), kv.ev0.data_ptr(),
+            kv.max_blocks, int(kv.sink), out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64x(out.stride()),
+            ws.data_ptr(), nbytes, _A._stream_handle(dev)), "lssab8_prefill_paged")
+    if check:
+        _A.check_device_errors(dev)
+    return out
+
+
+def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
+    """One decode step of a batch whose sequences share their first shared_len tokens (one system prompt):
+    q [B, H, dh] -> out [B, H, dh], bit-identical to decode(q, kv).
+
+    The first shared_len // 128 blocks must be the same pages, with the same exponents, in every live sequence
+    (length > 0); they are read and scored once for the batch instead of once a sequence.  Fewer than 128
+    shared tokens run decode.  A sequence that is shorter than the shared blocks, or does not hold the same
+    ones, raises RuntimeError (device error 16) when checked.  Batches with several prefixes: one call for
+    each."""
+    if q.dim() != 3:
+        raise ValueError("q must be [B, H, dh]")
+    B, H, dh = q.shape
+    shared_len = int(shared_len)
+    if shared_len < 0:
+        raise ValueError("shared_len must not be negative")
+    if shared_len < KB:
+        return decode(q, kv, out=out, out_dtype=out_dtype, check=check)
+    dev = _check_lattice(q, kv, B, H, dh)
+    if shared_len // KB > kv.max_blocks or shared_len // KB * (KB // PAGE) > kv.block_table.shape[1]:
+        raise ValueError("the lattice holds at most %d blocks a sequence" % kv.max_blocks)
+    if out is None:
+        out = torch.empty((B, H, dh), dtype=out_dtype or q.dtype, device=dev)
+    _check_out(out, (B, H, dh), dev)
+    L = _lib.load()
+    with torch.cuda.device(dev):
+        nbytes = L.lssab8_decode_shared_workspace_size(B, H, kv.KVH, dh, kv.max_blocks, shared_len)
+        if nbytes == 0:
+            raise ValueError("unsupported decode shape")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)       # a call's own, as in prefill_paged
+        _lib.check(L.lssab8_decode_shared(
+            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64x(q.stride()), B, H, kv.KVH, dh, kv.seq_lens.data_ptr(),
+            shared_len, kv.block_table.data_ptr(), kv.block_table.shape[1], kv.num_pages, kv.k8p.data_ptr(),
+            kv.v8p.data_ptr(), kv.ek.data_ptr(), kv.ev.data_ptr(), kv.ev0.data_ptr(), kv.max_blocks, int(kv.sink),
+            out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64x(out.stride()), ws.data_ptr(), nbytes,
+            _A._stream_handle(dev)), "lssab8_decode_shared")
+    if check:
+        _A.check_device_errors(dev)
+    return out

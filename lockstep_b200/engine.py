@@ -17,8 +17,12 @@ this library, in the engine's own terms:
     steps (as the reference's row verifier keys it, tools/verify_rows.py:63-104);
   * Lssab8Attention.forward(layer, query, key, value, k_cache, v_cache, meta) stores the step's new
     keys and values in the float cache, appends them to the lattice (lssab8_kv_append: only the
-    open block and new blocks are quantised), then runs each prompt chunk through the block-aligned
-    chunked prefill and every generated row through one split-KV decode call.
+    open block and new blocks are quantised), then runs the prompt rows of every sequence through one
+    packed prefill over the lattice (decode.prefill_paged) and every generated row through one
+    split-KV decode call;
+  * with a rotary plan (lockstep_b200.rotary) the queries and keys come unrotated and the float-cache
+    store rotates them (one launch); StepMeta.build makes a step's block table, slots and positions
+    on the device (lockstep_b200.paging) for an engine that keeps only request lengths.
 
 lockstep_b200.vllm_backend wraps this forward pass as a vLLM attention backend: its metadata
 builder supplies query_start_loc, seq_lens, block_table, slot_mapping and the scheduler's prefill
@@ -28,8 +32,9 @@ from dataclasses import dataclass
 
 import torch
 
-from . import attention as A
 from . import decode as D
+from . import paging as P
+from . import rotary as R
 
 PAGE = 16
 KB = 128
@@ -42,12 +47,36 @@ class StepMeta:
     query_start_loc [nseq + 1] (host ints): sequence i's new tokens are rows [qsl[i], qsl[i+1]);
     seq_lens [nseq] (host ints): each sequence's length after this step; block_table
     [nseq, max_pages] int32 (CUDA): the pages of each sequence; slot_mapping [ntok] int64 (CUDA):
-    page * 16 + row of each new token; is_prefill [nseq] (host bools): the scheduler's flag."""
+    page * 16 + row of each new token; is_prefill [nseq] (host bools): the scheduler's flag;
+    positions [ntok] (CUDA, int32 or int64): each new token's position, for an engine with a rotary
+    plan."""
     query_start_loc: list
     seq_lens: list
     block_table: torch.Tensor
     slot_mapping: torch.Tensor
     is_prefill: list
+    positions: torch.Tensor = None
+
+    @classmethod
+    def build(cls, lens, new_tokens, is_prefill, block_table, free_pages):
+        """The step in which sequence i grows from lens[i] by new_tokens[i] tokens (host ints).  The new pages
+        are the first entries of free_pages (int32, CUDA) in sequence order, written to block_table [nseq,
+        max_pages] (int32, CUDA) in place; returns (meta, number of free pages taken)."""
+        lens, new = [int(x) for x in lens], [int(x) for x in new_tokens]
+        if len(new) != len(lens) or len(is_prefill) != len(lens) or min(lens + new, default=0) < 0:
+            raise ValueError("lens, new_tokens and is_prefill must match, lengths must not be negative")
+        pages = lambda x: -(-x // PAGE)                      # noqa: E731
+        used = sum(pages(a + b) - pages(a) for a, b in zip(lens, new))
+        if used > free_pages.numel():
+            raise ValueError("the step needs %d pages, %d are free" % (used, free_pages.numel()))
+        dev = block_table.device
+        t = P.step_tables(torch.tensor(lens, dtype=torch.int32, device=dev),
+                          torch.tensor(new, dtype=torch.int32, device=dev), block_table, free_pages, sum(new))
+        qsl = [0]
+        for x in new:
+            qsl.append(qsl[-1] + x)
+        return cls(query_start_loc=qsl, seq_lens=[a + b for a, b in zip(lens, new)], block_table=block_table,
+                   slot_mapping=t.slot_mapping, is_prefill=list(is_prefill), positions=t.positions), used
 
 
 class LatticeLayer:
@@ -116,11 +145,12 @@ class Lssab8Attention:
     """LSSA-B8 (sink=False) / B9.1 sink_alone (sink=True) attention for a paged serving engine."""
 
     def __init__(self, num_heads, num_kv_heads, head_size, num_pages, max_len, max_seqs, num_layers=1, sink=False,
-                 device=None):
+                 device=None, rotary=None):
         if num_heads % num_kv_heads:
             raise ValueError("query heads must be a multiple of kv heads")
         self.H, self.KVH, self.dh = num_heads, num_kv_heads, head_size
         self.sink = bool(sink)
+        self.rotary = rotary                              # a rotary plan: queries and keys come unrotated
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
         self.layers = [LatticeLayer(num_pages, num_kv_heads, head_size, max_len, max_seqs, sink, dev)
                        for _ in range(num_layers)]
@@ -141,9 +171,14 @@ class Lssab8Attention:
             out = torch.empty_like(query)
         # 1. the step's keys and values into the engine's float cache (by page and row, so a cache
         #    whose pages are strided -- K and V interleaved per page -- is written in place)
-        page, row = meta.slot_mapping // PAGE, meta.slot_mapping % PAGE
-        k_cache[page, row] = key.to(k_cache.dtype)
-        v_cache[page, row] = value.to(v_cache.dtype)
+        if self.rotary is not None:
+            if meta.positions is None:
+                raise ValueError("an engine with a rotary plan needs the step's positions")
+            query = R.rotate_append(query, key, value, meta.positions, meta.slot_mapping, k_cache, v_cache, self.rotary)
+        else:
+            page, row = meta.slot_mapping // PAGE, meta.slot_mapping % PAGE
+            k_cache[page, row] = key.to(k_cache.dtype)
+            v_cache[page, row] = value.to(v_cache.dtype)
         # 2. the lattice: the open block and new blocks of every sequence, from the float cache
         bt = meta.block_table.to(device=dev, dtype=torch.int32)
         if bt.shape[1] < st.max_pages:
@@ -160,15 +195,22 @@ class Lssab8Attention:
         st.ek[sidx], st.ev[sidx], st.ev0[sidx] = kv.ek, kv.ev, kv.ev0
         for s, L in zip(slots, lens):
             st.lens[s] = L
-        # 3. prompt rows: block-aligned chunks of the causal prefill
+        # 3. prompt rows: every sequence's block-aligned chunk in one packed prefill over the lattice
+        prompts = [bool(meta.is_prefill[i]) and qlen[i] > 0 for i in range(nseq)]
         for i in range(nseq):
-            if not meta.is_prefill[i] or qlen[i] == 0:
-                continue
-            T0, T = before[i], lens[i]
-            if T0 % KB:
+            if prompts[i] and before[i] % KB:
                 raise ValueError("prompt chunk of sequence %d starts at %d, not a multiple of %d (the scheduler's "
-                                 "chunk alignment)" % (i, T0, KB))
-            out[qsl[i]:qsl[i + 1]] = self._prompt_rows(query[qsl[i]:qsl[i + 1]], k_cache, v_cache, bt[i], T0, T)
+                                 "chunk alignment)" % (i, before[i], KB))
+        if any(prompts):
+            cu = torch.tensor(qsl, dtype=torch.int32, device=dev)
+            act = torch.tensor(prompts, dtype=torch.bool, device=dev)
+            if out.dtype == query.dtype:
+                D.prefill_paged(query, kv, cu, active=act, out=out)
+            else:
+                rows = D.prefill_paged(query, kv, cu, active=act)
+                for i in range(nseq):
+                    if prompts[i]:
+                        out[qsl[i]:qsl[i + 1]] = rows[qsl[i]:qsl[i + 1]]
         # 4. generated rows: one split-KV decode over the lattice for every one-row sequence
         gen = [i for i in range(nseq) if not meta.is_prefill[i] and qlen[i] > 0]
         if any(qlen[i] != 1 for i in gen):
@@ -182,16 +224,3 @@ class Lssab8Attention:
                             max_blocks=st.max_blocks, num_pages=st.num_pages, sink=self.sink)
             out[rows] = D.decode(query[rows].contiguous(), dkv, out_dtype=query.dtype)
         return out
-
-    def _prompt_rows(self, q, k_cache, v_cache, bt_row, T0, T):
-        """Rows [T0, T) of one sequence's causal prefill: the chunk's queries against the lattice of
-        keys [0, T), gathered from the paged float cache."""
-        npg = (T + PAGE - 1) // PAGE
-        pages = bt_row[:npg].long()
-        kk = k_cache[pages].reshape(npg * PAGE, self.KVH, self.dh)[:T].transpose(0, 1)[None]
-        vv = v_cache[pages].reshape(npg * PAGE, self.KVH, self.dh)[:T].transpose(0, 1)[None]
-        q8, eq = A.quant_rows(q.transpose(0, 1)[None])
-        k8, ek, _ = A.quant_blocks(kk, 0)
-        v8, ev, ev0 = A.quant_blocks(vv, 2 if self.sink else 0)
-        o = A.prefill_chunk_lattice(q8, eq, k8, ek, v8, ev, ev0 if self.sink else None, T0, T, out_dtype=q.dtype)
-        return o[0]

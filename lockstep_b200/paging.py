@@ -1,0 +1,76 @@
+"""A serving step's tables, built on the device from its request lengths (host layer over the C ABI): query
+starts, lengths, the pages that new tokens need (from a free list, in sequence order), slots and positions.
+Nothing is read back, so a step can be captured in a CUDA graph and replayed with new lengths in the same
+buffers."""
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from . import attention as _A
+
+PAGE = 16
+MAX_SEQS = 16384
+
+
+@dataclass
+class StepTables:
+    """query_start_loc [n + 1] int32, seq_lens [n] int32 (after the step), slot_mapping [cap] int64, positions
+    [cap] int64, seq_index [cap] int32 (entries past the last token: -1, 0, -1), pages_used [1] int32 (entries
+    of the free list taken)."""
+    query_start_loc: torch.Tensor
+    seq_lens: torch.Tensor
+    slot_mapping: torch.Tensor
+    positions: torch.Tensor
+    seq_index: torch.Tensor
+    pages_used: torch.Tensor
+
+
+def alloc_step_tables(n, cap, device):
+    i32 = lambda *s: torch.empty(s, dtype=torch.int32, device=device)          # noqa: E731
+    i64 = lambda *s: torch.empty(s, dtype=torch.int64, device=device)          # noqa: E731
+    return StepTables(query_start_loc=i32(n + 1), seq_lens=i32(n), slot_mapping=i64(cap), positions=i64(cap),
+                      seq_index=i32(cap), pages_used=i32(1))
+
+
+def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None, check=True):
+    """Tables of a step in which sequence i grows from lens[i] by new_tokens[i] tokens (both [n] int32, CUDA).
+
+    block_table [n, max_pages] int32 is updated in place with the new pages, which are the first entries of
+    free_pages [F] int32 in sequence order; its other entries stay.  max_tokens: length of the token arrays
+    (at least the step's tokens).  out: tables of an earlier call with the same n and max_tokens, rewritten.
+    Lengths that do not fit raise RuntimeError (device error 16) when checked."""
+    dev = _A._require_cuda(lens, new_tokens, block_table, free_pages)
+    n = lens.numel()
+    for t, name in ((lens, "lens"), (new_tokens, "new_tokens"), (block_table, "block_table"), (free_pages, "free_pages")):
+        if t.dtype != torch.int32:
+            raise TypeError("%s must be int32, got %s" % (name, t.dtype))
+    if lens.dim() != 1 or new_tokens.shape != lens.shape or not 0 < n <= MAX_SEQS:
+        raise ValueError("lens and new_tokens must be [n], n from 1 to %d" % MAX_SEQS)
+    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] == 0 or free_pages.dim() != 1:
+        raise ValueError("block_table must be [n, max_pages], free_pages [F]")
+    if block_table.stride(1) != 1 or block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_table rows must be contiguous and apart")
+    cap = int(max_tokens)
+    if not 0 <= cap < 1 << 31:
+        raise ValueError("max_tokens must be from 0 to 2^31 - 1")
+    lens, new_tokens, free_pages = lens.contiguous(), new_tokens.contiguous(), free_pages.contiguous()
+    if out is None:
+        out = alloc_step_tables(n, cap, dev)
+    else:
+        want = alloc_step_tables(n, cap, "meta")
+        for f in StepTables.__dataclass_fields__:
+            t, w = getattr(out, f), getattr(want, f)
+            if t.shape != w.shape or t.dtype != w.dtype or t.device != dev or not t.is_contiguous():
+                raise ValueError("out: tables of another step shape (%s)" % f)
+        if out.seq_lens.data_ptr() in (lens.data_ptr(), new_tokens.data_ptr()):
+            raise ValueError("out.seq_lens must not be the step's own lens or new_tokens")
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().lssab8_step_tables(
+            lens.data_ptr(), new_tokens.data_ptr(), n, block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], free_pages.data_ptr() if free_pages.numel() else None, free_pages.numel(), cap,
+            out.query_start_loc.data_ptr(), out.seq_lens.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(),
+            out.seq_index.data_ptr(), out.pages_used.data_ptr(), _A._stream_handle(dev)), "lssab8_step_tables")
+    if check:
+        _A.check_device_errors(dev)
+    return out

@@ -1,0 +1,196 @@
+"""Rotary positions (host layer over the C ABI): the rotation of queries and keys before the contract's
+quantisers, its inverse (the gradient), and a serving step's fused form that also stores the new keys and
+values in the engine's paged float cache.
+
+    plan = make_plan(128, scaling={"kind": "bands", "factor": 32.0, "original": 8192})
+    q = rotate(q, positions, plan)                      # [B, H, T, dh] or [N, H, dh]
+    q = rotate_append(q, k, v, positions, slot_mapping, k_cache, v_cache, plan)
+
+theta_i = base^(-2 i / rotary_dim) for pair i, scaled for long contexts by one of
+    {"kind": "linear", "factor": s}         theta / s
+    {"kind": "ntk", "factor": s}            base s^(d / (d - 2)), d = rotary_dim
+    {"kind": "bands", "factor": s, "original": L0, "fast": 32.0, "slow": 1.0, "attention": m}
+        pairs that turn more than `fast` times over L0 positions keep theta, those below `slow` turns take
+        theta / s, in between linearly in the turns; cosine and sine times m (default 0.1 ln s + 1)
+The angle of position p is p theta_i, kept as an exact fraction of a turn (64-bit integer arithmetic), so it
+is as good at position 10^6 as at 1.
+"""
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from . import attention as _A
+
+PAGE = 16
+_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+@dataclass
+class RotaryPlan:
+    """freq [rotary_dim / 2] int64 on the device: theta_i / (2 pi) in 2^-64 turns."""
+    freq: torch.Tensor
+    factor: float
+    head_dim: int
+    rotary_dim: int
+    layout: str
+
+
+def frequencies(rotary_dim, base=10000.0, scaling=None):
+    """(theta_i as Python floats, the factor on cosine and sine)."""
+    d, factor = int(rotary_dim), 1.0
+    kind = None if scaling is None else scaling.get("kind")
+    if scaling is not None and kind not in ("linear", "ntk", "bands"):
+        raise ValueError("scaling kind must be linear, ntk or bands, got %r" % (kind,))
+    s = 1.0 if scaling is None else float(scaling["factor"])
+    if not (s > 0.0 and math.isfinite(s)) or not (base > 0.0 and math.isfinite(base)):
+        raise ValueError("base and scaling factor must be positive")
+    if kind == "ntk" and d > 2:
+        base = base * s ** (d / (d - 2))
+    theta = [base ** (-i / d) for i in range(0, d, 2)]
+    if kind == "linear":
+        theta = [t / s for t in theta]
+    if kind == "bands":
+        L0, fast, slow = float(scaling["original"]), float(scaling.get("fast", 32.0)), float(scaling.get("slow", 1.0))
+        if not (L0 > 0 and fast > slow):
+            raise ValueError("bands need original > 0 and fast > slow")
+        keep = [min(1.0, max(0.0, (L0 * t / (2 * math.pi) - slow) / (fast - slow))) for t in theta]
+        theta = [t * k + t / s * (1 - k) for t, k in zip(theta, keep)]
+        m = scaling.get("attention")
+        factor = float(m) if m is not None else (0.1 * math.log(s) + 1.0 if s > 1 else 1.0)
+    return theta, factor
+
+
+def make_plan(head_dim, rotary_dim=None, base=10000.0, layout="half", scaling=None, device=None):
+    """The plan of a model's rotary positions: made once, kept by the caller, shared by its layers."""
+    rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
+    if not 0 < head_dim <= 512 or not 0 < rotary_dim <= head_dim or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even and at most head_dim, head_dim at most 512")
+    if layout not in _LAYOUTS:
+        raise ValueError("layout must be half or interleaved, got %r" % (layout,))
+    theta, factor = frequencies(rotary_dim, base, scaling)
+    turns = [int(round(t / (2 * math.pi) * 2.0 ** 64)) % (1 << 64) for t in theta]
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    freq = torch.tensor([u - (1 << 64) if u >= 1 << 63 else u for u in turns], dtype=torch.int64).to(dev)
+    return RotaryPlan(freq=freq, factor=factor, head_dim=int(head_dim), rotary_dim=rotary_dim, layout=layout)
+
+
+def _check_positions(positions):
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be int32 or int64, got %s" % positions.dtype)
+
+
+def _written_once(t):
+    """No two elements of t share memory (as far as strides tell)."""
+    dims = sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1)
+    end = 0
+    for st, n in dims:
+        if st <= end:
+            return False
+        end += st * (n - 1)
+    return True
+
+
+def _launch(x, positions, plan, inverse, out):
+    dev = _A._require_cuda(x, positions, plan.freq, out)
+    if x.numel() == 0:
+        return out
+    x4, y4 = (x, out) if x.dim() == 4 else (x.transpose(0, 1)[None], out.transpose(0, 1)[None])
+    B, H, T, dh = x4.shape
+    ps = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().lssab8_rotate(
+            x4.data_ptr(), _A.dtype_code(x.dtype), B, H, T, dh, _lib.i64x(x4.stride()), positions.data_ptr(),
+            int(positions.dtype == torch.int64), _lib.i64x(ps), plan.freq.data_ptr(), plan.factor, plan.rotary_dim,
+            _LAYOUTS[plan.layout], int(bool(inverse)), y4.data_ptr(), _lib.i64x(y4.stride()), _A._stream_handle(dev)),
+            "lssab8_rotate")
+    return out
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, plan, inverse):
+        ctx.save_for_backward(positions)
+        ctx.plan, ctx.inverse = plan, inverse
+        return _launch(x, positions, plan, inverse, torch.empty_like(x, memory_format=torch.preserve_format))
+
+    @staticmethod
+    def backward(ctx, g):
+        positions, = ctx.saved_tensors
+        return rotate(g, positions, ctx.plan, inverse=not ctx.inverse), None, None, None
+
+
+def rotate(x, positions, plan, inverse=False, out=None):
+    """x [B, H, T, dh] with positions [T] or [B, T], or x [N, H, dh] with positions [N] -> rotated x, same type
+    and shape (any strides; float32, float16, bfloat16).  inverse=True: the transposed map (it undoes
+    the rotation when the plan's factor is 1); differentiable in x, the gradient being the other direction.
+    out: written instead (out=x rotates in place); not with a gradient."""
+    if x.dim() not in (3, 4) or x.shape[-1] != plan.head_dim:
+        raise ValueError("x must be [B, H, T, %d] or [N, H, %d], got %s" % (plan.head_dim, plan.head_dim, tuple(x.shape)))
+    _check_positions(positions)
+    want = [(x.shape[0],)] if x.dim() == 3 else [(x.shape[2],), (x.shape[0], x.shape[2])]
+    if tuple(positions.shape) not in want:
+        raise ValueError("positions must be %s, got %s" % (" or ".join(map(str, want)), tuple(positions.shape)))
+    _A.dtype_code(x.dtype)
+    if torch.is_grad_enabled() and x.requires_grad:
+        if out is not None:
+            raise ValueError("out= has no gradient: rotate a detached tensor, or leave out away")
+        return _Rotate.apply(x, positions, plan, bool(inverse))
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.preserve_format)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("out must have x's shape and dtype")
+    if not _written_once(out):
+        raise ValueError("out has elements that share memory")
+    return _launch(x, positions, plan, inverse, out)
+
+
+def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, plan, out=None, check=True):
+    """A serving step's new tokens: query [N, H, dh] rotated (returned, or written to out, which may be
+    query), key [N, KVH, dh] rotated and value [N, KVH, dh] stored in k_cache / v_cache [num_pages, 16, KVH, dh]
+    (any page, row and head strides; the cache's own dtype, one rounding) at slot_mapping [N] int64, page * 16 +
+    row.  Slot -1 stores nothing.  Inference only: no gradient flows through it."""
+    dev = _A._require_cuda(query, key, value, positions, slot_mapping, k_cache, v_cache, plan.freq)
+    if query.dim() != 3 or key.dim() != 3 or key.shape != value.shape or key.shape[0] != query.shape[0]:
+        raise ValueError("query must be [N, H, dh], key and value [N, KVH, dh]")
+    if not query.dtype == key.dtype == value.dtype or k_cache.dtype != v_cache.dtype:
+        raise TypeError("query, key and value must share one dtype, and so must the caches")
+    N, H, dh = query.shape
+    KVH = key.shape[1]
+    if dh != plan.head_dim or key.shape[2] != dh:
+        raise ValueError("the plan is for head dim %d" % plan.head_dim)
+    if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or tuple(k_cache.shape[1:]) != (PAGE, KVH, dh)):
+        raise ValueError("caches must be [num_pages, 16, %d, %d]" % (KVH, dh))
+    _check_positions(positions)
+    if tuple(positions.shape) != (N,) or tuple(slot_mapping.shape) != (N,):
+        raise ValueError("positions and slot_mapping must be [%d]" % N)
+    if slot_mapping.dtype != torch.int64:
+        raise TypeError("slot_mapping must be int64")
+    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+        raise ValueError("rotate_append has no gradient (use rotate)")
+    if out is None:
+        out = torch.empty((N, H, dh), dtype=query.dtype, device=dev)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev:
+        raise ValueError("out must have the query's shape, dtype and device")
+    for t in (query, key, value, k_cache, v_cache, out):
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise ValueError("channels must be contiguous")
+    for t in (out, k_cache, v_cache):
+        if not _written_once(t):
+            raise ValueError("out and the caches must not have elements that share memory")
+    if N == 0:
+        return out
+    slot_mapping = slot_mapping.contiguous()
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().lssab8_rotate_append(
+            query.data_ptr(), key.data_ptr(), value.data_ptr(), _A.dtype_code(query.dtype), N, H, KVH, dh,
+            _lib.i64x(query.stride()[:2]), _lib.i64x(key.stride()[:2]), _lib.i64x(value.stride()[:2]),
+            positions.data_ptr(), int(positions.dtype == torch.int64), positions.stride(0), plan.freq.data_ptr(),
+            plan.factor, plan.rotary_dim, _LAYOUTS[plan.layout], out.data_ptr(), _lib.i64x(out.stride()[:2]),
+            k_cache.data_ptr(), v_cache.data_ptr(), _A.dtype_code(k_cache.dtype), _lib.i64x(k_cache.stride()[:3]),
+            _lib.i64x(v_cache.stride()[:3]), k_cache.shape[0], slot_mapping.data_ptr(), _A._stream_handle(dev)),
+            "lssab8_rotate_append")
+    if check:
+        _A.check_device_errors(dev)
+    return out
