@@ -4,6 +4,7 @@ There is no fallback: if the library is missing or fails to load, importing the 
 modules raises, so no caller can silently run a non-native path.
 """
 import ctypes
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -106,6 +107,12 @@ def version():
     buf = ctypes.create_string_buffer(160)
     check(load().lssab8_version(buf, len(buf)), "lssab8_version")
     return buf.value.decode()
+
+
+@functools.lru_cache(maxsize=4096)
+def i64c(vals):
+    """i64x of a tuple, kept: strides recur call after call, and the library only reads them."""
+    return (ctypes.c_int64 * len(vals))(*vals)
 
 
 def i64x(vals):

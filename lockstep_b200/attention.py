@@ -22,17 +22,36 @@ def dtype_code(dt):
 
 
 def _stream_handle(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)      # current_stream(device).cuda_stream, 2.6 us cheaper
+
+
+class _Here:
+    """The device is current already."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """torch.cuda.device(device), without its cost when the device is current already."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _require_cuda(*ts):
     for t in ts:
-        if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError("LSSA-B8 on B200 needs CUDA tensors (no CPU fallback exists)")
-    dev = ts[0].device
-    if any(t.device != dev for t in ts):
-        raise ValueError("all tensors must be on the same CUDA device")
-    return dev
+    i = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != i:
+            raise ValueError("all tensors must be on the same CUDA device")
+    return ts[0].device
 
 
 def tpad(T):

@@ -342,28 +342,6 @@ static int prefill_lattice_impl(const int8_t* q8, const int32_t* eq, const int8_
               : launch_prefill_out<64, false>(out_dtype, tq, tk, tv, a, ds->num_sms, st);
 }
 
-// The decode's query quantiser ([B, H, dh] rows): the vector kernel is launched with
-// programmatic dependent launch, so it runs beside the decode plan kernel before it (which it does
-// not read); it waits for the plan before it completes, so the streaming kernel's wait on it
-// covers the plan too.  Other layouts take lssab8_quant_rows.
-int lssab8::quant_queries_pdl(const void* q, int dtype, int B, int H, int dh, const int64_t* q4, int8_t* q8,
-                              int32_t* eq, cudaStream_t st) {
-  Strides4 s{q4[0], q4[1], q4[2], q4[3]};
-  return with_in_dtype(dtype, [&](auto tag) -> int {
-    using InT = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
-    if (!vec_ok<InT>(q, s, dh)) return lssab8_quant_rows(q, dtype, B, H, 1, dh, q4, 1, q8, eq, st);
-    constexpr int N = Vec16<InT>::kN;
-    const int rpw = 32 / (dh / N);
-    const long long per_cta = 8LL * rpw * kRowsPerLane;
-    const int grid = (int)(((long long)B * H + per_cta - 1) / per_cta);
-    if (dh == 128)
-      return launch_pdl(quant_rows_vec_kernel<InT, 128>, dim3(grid), dim3(256), 0, st, static_cast<const InT*>(q), s, B,
-                        H, 1, 1, q8, eq);
-    return launch_pdl(quant_rows_vec_kernel<InT, 64>, dim3(grid), dim3(256), 0, st, static_cast<const InT*>(q), s, B, H,
-                      1, 1, q8, eq);
-  });
-}
-
 // ========================================================================== extern "C"
 extern "C" {
 
@@ -410,6 +388,28 @@ int lssab8_device_errors(int clear, void* stream, int* bits) {
     if (cudaStreamSynchronize(s) != cudaSuccess) return kErrCuda;
   }
   return kOk;
+}
+
+// The decode's query quantiser ([B, H, dh] rows): the vector kernel is launched with
+// programmatic dependent launch, so it runs beside the decode plan kernel before it (which it does
+// not read); it waits for the plan before it completes, so the streaming kernel's wait on it
+// covers the plan too.  Other layouts take lssab8_quant_rows.
+static int quant_queries_pdl(const void* q, int dtype, int B, int H, int dh, const int64_t* q4, int8_t* q8,
+                             int32_t* eq, cudaStream_t st) {
+  Strides4 s{q4[0], q4[1], q4[2], q4[3]};
+  return with_in_dtype(dtype, [&](auto tag) -> int {
+    using InT = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
+    if (!vec_ok<InT>(q, s, dh)) return lssab8_quant_rows(q, dtype, B, H, 1, dh, q4, 1, q8, eq, st);
+    constexpr int N = Vec16<InT>::kN;
+    const int rpw = 32 / (dh / N);
+    const long long per_cta = 8LL * rpw * kRowsPerLane;
+    const int grid = (int)(((long long)B * H + per_cta - 1) / per_cta);
+    if (dh == 128)
+      return launch_pdl(quant_rows_vec_kernel<InT, 128>, dim3(grid), dim3(256), 0, st, static_cast<const InT*>(q), s, B,
+                        H, 1, 1, q8, eq);
+    return launch_pdl(quant_rows_vec_kernel<InT, 64>, dim3(grid), dim3(256), 0, st, static_cast<const InT*>(q), s, B, H,
+                      1, 1, q8, eq);
+  });
 }
 
 int lssab8_quant_rows(const void* x, int dtype, int B, int H, int T, int dh, const int64_t* xs, int Tpad,
@@ -791,11 +791,10 @@ int lssab8_decode(const void* q, int dtype, const int64_t* qs, int B, int H, int
   // (the ticket reset and the plan come first so the query quantiser directly precedes the
   // decode kernel, which may then start under programmatic dependent launch)
   if (dh == 128) {                                   // the live-block plan; it also zeroes the tickets
-    decode_plan_kernel<false><<<1, kPlanThreads, 0, s>>>(seq_lens, B, max_blocks, max_pages,
+    decode_plan_kernel<><<<1, kPlanThreads, 0, s>>>(seq_lens, B, max_blocks, max_pages,
                                                   reinterpret_cast<int*>(base + w.blk_off),
                                                   reinterpret_cast<int*>(base + w.order),
-                                                  reinterpret_cast<unsigned int*>(base + w.tickets), B * KVH, ds->err,
-                                                  0, nullptr);
+                                                  reinterpret_cast<unsigned int*>(base + w.tickets), B * KVH, ds->err);
     if ((rc = launch_rc())) return rc;
   } else if (cudaMemsetAsync(base + w.tickets, 0, (size_t)B * KVH * 4, s) != cudaSuccess) {
     return kErrCuda;
@@ -872,11 +871,10 @@ int lssab8_decode_noalloc(const void* q, int dtype, const int64_t* qs, int B, in
   // and the plan come first, as in lssab8_decode, so the query quantiser directly precedes the
   // decode kernel
   if (dh == 128) {                                   // the live-block plan; it also zeroes the tickets
-    decode_plan_kernel<false><<<1, kPlanThreads, 0, s>>>(seq_lens, B, max_blocks, max_pages,
+    decode_plan_kernel<><<<1, kPlanThreads, 0, s>>>(seq_lens, B, max_blocks, max_pages,
                                                   reinterpret_cast<int*>(base + w.blk_off),
                                                   reinterpret_cast<int*>(base + w.order),
-                                                  reinterpret_cast<unsigned int*>(base + w.tickets), B * KVH, ds->err,
-                                                  0, nullptr);
+                                                  reinterpret_cast<unsigned int*>(base + w.tickets), B * KVH, ds->err);
     if ((rc = launch_rc())) return rc;
   } else if (cudaMemsetAsync(base + w.tickets, 0, (size_t)B * KVH * 4, s) != cudaSuccess) {
     return kErrCuda;

@@ -139,7 +139,8 @@ __device__ __forceinline__ void decode_merge_head(const DecodeArgs& p, int b, in
 }
 
 // SHARED: only the blocks after the shared ones, whose partials alone are stored (the refold is
-// decode_merge_kernel, decode_tc.cuh).
+// decode_merge_kernel, decode_tc.cuh).  It runs beside the shared-prefix kernel before it, and completes after it
+// (every CTA's wait), so that the refold's wait covers both.
 template <int DH, bool SINK, typename OutT, bool SHARED = false>
 __global__ void __launch_bounds__(128)
 decode_kernel(const DecodeArgs p) {
@@ -161,9 +162,14 @@ decode_kernel(const DecodeArgs p) {
   const int nblk = (L_len + kKB - 1) / kKB;
   const int first = SHARED ? p.skip_blocks : 0;
   const int nsplit = (nblk - first + p.split_blocks - 1) / p.split_blocks;
-  if (L_len <= 0 || split >= nsplit) return;
+  if (SHARED) pdl_launch_dependents();
+  if (L_len <= 0 || split >= nsplit) {
+    if (SHARED) pdl_wait();
+    return;
+  }
   if (nblk > p.max_blocks || (L_len + 15) / 16 > p.max_pages) {   // lattice arrays too short
     if (tid == 0) atomicOr(p.err, kDevBadPage);
+    if (SHARED) pdl_wait();
     return;
   }
   const int blo = first + split * p.split_blocks;
@@ -312,7 +318,10 @@ decode_kernel(const DecodeArgs p) {
     if (tid == 0 && blk + 2 < bhi) issue(blk + 2, s);
   }
 
-  if (SHARED) return;
+  if (SHARED) {
+    pdl_wait();
+    return;
+  }
   // ---- ticket: the last split of this (sequence, kv head) merges, in ascending block order
   __threadfence();
   __syncthreads();

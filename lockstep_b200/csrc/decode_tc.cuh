@@ -72,16 +72,19 @@ constexpr int kDecChunk = 8;                       // blocks per scheduling chun
 // sequence of v is found by advancing one cursor over off (each CTA reads off once).  Sequences
 // the plan found too long for the lattice arrays have no live blocks (and are flagged there).
 // Every role runs its own copy and sees the same sequence of blocks.
-// SHARED: the list holds the blocks after the skip_blocks shared ones only.
+// SHARED: the list holds the blocks after the skip_blocks shared ones only, and may be short: its chunks shrink
+// until every CTA has one.
 template <bool SHARED> struct DecIter {
   int v, vend, chunk, nchunks, total;
+  int len;                                         // blocks a chunk
   int cur_b, lo, hi, nb, L;                        // this sequence's live range [lo, hi) of v
   __device__ __forceinline__ void init(const DecodeArgs& p) {
     total = p.KVH * __ldg(&p.blk_off[p.B]);
-    nchunks = (total + kDecChunk - 1) / kDecChunk;
+    len = SHARED ? max(1, min(kDecChunk, (total + (int)gridDim.x - 1) / (int)gridDim.x)) : kDecChunk;
+    nchunks = (total + len - 1) / len;
     chunk = blockIdx.x;
-    v = chunk * kDecChunk;
-    vend = min(v + kDecChunk, total);
+    v = chunk * len;
+    vend = min(v + len, total);
     cur_b = 0;
     lo = 0;
     nb = __ldg(&p.blk_off[1]);
@@ -92,8 +95,8 @@ template <bool SHARED> struct DecIter {
     if (v >= vend) {
       chunk += gridDim.x;
       if (chunk >= nchunks) return false;
-      v = chunk * kDecChunk;
-      vend = min(v + kDecChunk, total);
+      v = chunk * len;
+      vend = min(v + len, total);
     }
     while (v >= hi) {                              // v < total, so some later sequence holds it
       ++cur_b;
@@ -117,21 +120,19 @@ template <bool SHARED> struct DecIter {
 // sequence that does not hold them sets kDevPlan, and *leader gets the first live sequence (-1: none).
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSortMax = 1024;                 // batches up to this size get the longest-first order
-template <bool SHARED>
-__global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const int32_t* seq_lens, int B, int max_blocks,
-                                                                    int max_pages, int* blk_off, int* order,
-                                                                    unsigned int* tickets, int nticket, int* err,
-                                                                    int skip_blocks, int* leader) {
+template <bool SHARED, int NT>
+__device__ __forceinline__ void decode_plan(const int32_t* seq_lens, int B, int max_blocks, int max_pages, int* blk_off,
+                                            int* order, unsigned int* tickets, int nticket, int* err, int skip_blocks,
+                                            int* leader) {
   __shared__ int lead;
-  __shared__ int warp_sums[kPlanThreads / 32];
+  __shared__ int warp_sums[NT / 32];
   __shared__ int carry;
   __shared__ int sl[kPlanSortMax];
-  pdl_launch_dependents();                         // the query quantiser runs beside the plan
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  for (int i = tid; i < nticket; i += kPlanThreads) tickets[i] = 0u;
+  for (int i = tid; i < nticket; i += NT) tickets[i] = 0u;
   if (tid == 0) { carry = 0; lead = INT32_MAX; }
   __syncthreads();
-  for (int base = 0; base < B; base += kPlanThreads) {
+  for (int base = 0; base < B; base += NT) {
     const int i = base + tid;
     int nb = 0;
     if (i < B) {
@@ -159,37 +160,44 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const int32_t
     if (lane == 31) warp_sums[w] = x;
     __syncthreads();
     if (w == 0) {
-      int ws = warp_sums[lane];
+      int ws = lane < NT / 32 ? warp_sums[lane] : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, ws, o);
         if (lane >= o) ws += y;
       }
-      warp_sums[lane] = ws;                        // inclusive over warps
+      if (lane < NT / 32) warp_sums[lane] = ws;    // inclusive over warps
     }
     __syncthreads();
     const int before = carry + (w > 0 ? warp_sums[w - 1] : 0) + x - nb;
     if (i < B) blk_off[i] = before;
     __syncthreads();
-    if (tid == 0) carry += warp_sums[kPlanThreads / 32 - 1];
+    if (tid == 0) carry += warp_sums[NT / 32 - 1];
     __syncthreads();
   }
   // the refold's sequence order, longest first (ties by index): order[rank(i)] = i with
   // rank(i) = #{j : L_j > L_i, or L_j == L_i and j < i}; larger batches keep the index order
   if (B <= kPlanSortMax) {
-    for (int i = tid; i < B; i += kPlanThreads) sl[i] = seq_lens[i];
+    for (int i = tid; i < B; i += NT) sl[i] = seq_lens[i];
     __syncthreads();
-    for (int i = tid; i < B; i += kPlanThreads) {
+    for (int i = tid; i < B; i += NT) {
       const int Li = sl[i];
       int r = 0;
       for (int j = 0; j < B; ++j) r += (sl[j] > Li || (sl[j] == Li && j < i)) ? 1 : 0;
       order[r] = i;
     }
   } else {
-    for (int i = tid; i < B; i += kPlanThreads) order[i] = i;
+    for (int i = tid; i < B; i += NT) order[i] = i;
   }
   if (tid == 0) blk_off[B] = carry;
   if (SHARED && tid == 0) *leader = lead == INT32_MAX ? -1 : lead;
+}
+template <int = 0>                                 // (a template: two translation units include it)
+__global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const int32_t* seq_lens, int B, int max_blocks,
+                                                                    int max_pages, int* blk_off, int* order,
+                                                                    unsigned int* tickets, int nticket, int* err) {
+  pdl_launch_dependents();                         // the query quantiser runs beside the plan
+  decode_plan<false, kPlanThreads>(seq_lens, B, max_blocks, max_pages, blk_off, order, tickets, nticket, err, 0, nullptr);
 }
 
 __device__ __forceinline__ uint32_t redux_max_s32(int v) {
@@ -250,7 +258,9 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();                             // the refold kernel may queue up behind us
-  pdl_wait();                                          // the plan and the query quantiser are complete
+  // the plan and the query quantiser are complete.  (SHARED: the shared-prefix kernel before this one let it
+  // start after its own wait for them; it does not read that kernel's output and runs beside it.)
+  if (!SHARED) pdl_wait();
 
   if (warp == 0) {
     // ================================================================ TMA producer
@@ -476,6 +486,7 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   }
 
   // ---- teardown
+  if (SHARED) pdl_wait();                              // this grid completes after the shared-prefix kernel, so the refold's wait covers both
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

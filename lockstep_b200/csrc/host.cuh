@@ -25,11 +25,6 @@ struct DevState {
 __attribute__((visibility("hidden"))) int dev_state(DevState** out);
 // cuTensorMapEncodeTiled, looked up in the driver once (null: not found).
 __attribute__((visibility("hidden"))) PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
-// The decode's query quantiser ([B, H, dh] rows) beside the plan kernel before it.
-__attribute__((visibility("hidden"))) int quant_queries_pdl(const void* q, int dtype, int B, int H, int dh,
-                                                            const int64_t* q4, int8_t* q8, int32_t* eq,
-                                                            cudaStream_t st);
-
 // rows x dh int8 matrix, box 128 rows x dh, swizzle = dh bytes
 // 2-D int8 tensor map over [rows, dh] (row pitch dh bytes), boxes of box_rows x dh, swizzled for
 // the UMMA K-major layouts (128B swizzle at dh 128, 64B at dh 64).

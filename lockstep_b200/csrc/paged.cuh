@@ -1,12 +1,14 @@
-// Attention over the paged lattice for whole steps: the plan of the packed prompt rows.  (Their kernel,
+// Attention over the paged lattice for whole steps: the plan of the packed prompt rows, and the launch that
+// plans a call and quantises its queries.  (Their kernel,
 // and the shared-prefix kernel, are prefill_kernel's paged forms, prefill.cuh; a shared batch's own
 // blocks and refold are the decode kernels' SHARED forms.)
 #pragma once
-#include "common.cuh"
+#include "decode_tc.cuh"
+#include "prep.cuh"
 
 namespace lssab8 {
 
-constexpr int kRowsPlanThreads = 1024;
+constexpr int kStepPlanThreads = 256;
 constexpr int kRowsPlanBins = 2048;
 
 struct RowsPlanArgs {
@@ -28,11 +30,11 @@ struct RowsPlanArgs {
 // shared memory; tiles of equal length fall in any order, which changes no result.  A sequence whose
 // rows do not fit (off the 128 grid, more rows than keys, a prefix past its end, past the lattice
 // arrays) gets no tiles and sets a device error.
-__global__ void __launch_bounds__(kRowsPlanThreads) rows_plan_kernel(const RowsPlanArgs p) {
-  __shared__ int ws[32];
+__device__ __forceinline__ void rows_plan(const RowsPlanArgs& p) {
+  constexpr int NT = kStepPlanThreads, NW = NT / 32;
+  __shared__ int ws[NW];
   __shared__ int carry;
   __shared__ int bins[kRowsPlanBins];
-  pdl_launch_dependents();                       // the query quantiser runs beside the plan
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   auto rows_of = [&](int b, int& n, int& T0, int& P) -> bool {
     n = 0;
@@ -46,9 +48,9 @@ __global__ void __launch_bounds__(kRowsPlanThreads) rows_plan_kernel(const RowsP
     return true;
   };
   if (tid == 0) carry = 0;
-  for (int i = tid; i < kRowsPlanBins; i += kRowsPlanThreads) bins[i] = 0;
+  for (int i = tid; i < kRowsPlanBins; i += NT) bins[i] = 0;
   __syncthreads();
-  for (int base = 0; base < p.B; base += kRowsPlanThreads) {
+  for (int base = 0; base < p.B; base += NT) {
     const int b = base + tid;
     int nt = 0;
     if (b < p.B) {
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(kRowsPlanThreads) rows_plan_kernel(const RowsP
     if (lane == 31) ws[w] = x;
     __syncthreads();
     int before = carry, all = 0;
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < NW; ++i) {
       if (i < w) before += ws[i];
       all += ws[i];
     }
@@ -97,15 +99,17 @@ __global__ void __launch_bounds__(kRowsPlanThreads) rows_plan_kernel(const RowsP
     key = kRowsPlanBins - min(nb, kRowsPlanBins);      // longest first
     return make_int4(lo, kt, nb, p.cu_q[lo] + t * 128);
   };
-  for (int e = tid; e < total; e += kRowsPlanThreads) {
+  for (int e = tid; e < total; e += NT) {
     int key;
     tile_at(e, key);
     atomicAdd(&bins[key], 1);
   }
   __syncthreads();
-  // exclusive scan of the bins, two a thread
-  const int a = bins[2 * tid], c = bins[2 * tid + 1];
-  int x = a + c;
+  // exclusive scan of the bins, consecutive ones a thread
+  constexpr int PB = kRowsPlanBins / NT;
+  int n = 0;
+  for (int i = 0; i < PB; ++i) n += bins[PB * tid + i];
+  int x = n;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
@@ -113,16 +117,89 @@ __global__ void __launch_bounds__(kRowsPlanThreads) rows_plan_kernel(const RowsP
   }
   if (lane == 31) ws[w] = x;
   __syncthreads();
-  int before = 0;
+  int before = x - n;
   for (int i = 0; i < w; ++i) before += ws[i];
-  bins[2 * tid] = before + x - a - c;
-  bins[2 * tid + 1] = before + x - c;
+  for (int i = 0; i < PB; ++i) {
+    const int c = bins[PB * tid + i];
+    bins[PB * tid + i] = before;
+    before += c;
+  }
   __syncthreads();
-  for (int e = tid; e < total; e += kRowsPlanThreads) {
+  for (int e = tid; e < total; e += NT) {
     int key;
     const int4 t = tile_at(e, key);
     p.tiles[atomicAdd(&bins[key], 1)] = t;
   }
+}
+
+// The plan of a call and the query quantiser in one launch: CTA 0 plans, the others quantise rows of q.  (They
+// do not read each other; as two kernels the small calls paid one more launch, 4 us of host time.)
+struct SharedPlanArgs {
+  const int32_t* seq_lens;
+  int B, max_blocks, max_pages;
+  int *blk_off, *order, *err;
+  int shared_blocks;
+  int* leader;
+};
+__device__ __forceinline__ void step_plan(const RowsPlanArgs& p) { rows_plan(p); }
+__device__ __forceinline__ void step_plan(const SharedPlanArgs& p) {
+  decode_plan<true, kStepPlanThreads>(p.seq_lens, p.B, p.max_blocks, p.max_pages, p.blk_off, p.order, nullptr, 0, p.err,
+                                      p.shared_blocks, p.leader);
+}
+template <typename Plan>
+__global__ void __launch_bounds__(kStepPlanThreads) step_plan_kernel(const Plan plan) {
+  pdl_launch_dependents();
+  step_plan(plan);
+}
+// P1 over tokens [N, H, dh] (strides 0, token, head; contiguous channels, 16-byte rows): row n H + h of q8 and eq.
+// quant_rows_vec's rule with fewer instructions, which bound it here (16,700 tokens of 32 heads: 53 us with its 64-bit
+// row divisions and a conversion an element): the maximum on the bit patterns, and clamp(rint(x 2^e), +-127) as one
+// fused multiply-add onto 1.5 2^23, whose low byte is the rounded integer, clamped as a float (NaN gives -127
+// there and here).
+template <typename InT, int DH>
+__device__ __forceinline__ void quant_tokens(int cta, const InT* __restrict__ x, Strides4 xs, int rows, int H,
+                                             int8_t* __restrict__ q8, int32_t* __restrict__ eq) {
+  constexpr int N = 16 / (int)sizeof(InT), G = DH / N, RPW = 32 / G, RPC = 8 * RPW;
+  const int sub = threadIdx.x % G;
+  const int row0 = cta * RPC * kRowsPerLane + threadIdx.x / G;
+  const bool flat = xs.s1 == H * xs.s2;                  // consecutive rows a head stride apart
+  uint4 u[kRowsPerLane];
+#pragma unroll
+  for (int k = 0; k < kRowsPerLane; ++k) {
+    const int row = row0 + k * RPC;
+    const int n = flat ? 0 : row / H;
+    u[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < rows) u[k] = __ldg(reinterpret_cast<const uint4*>(x + n * xs.s1 + (row - n * H) * xs.s2 + sub * N));
+  }
+#pragma unroll
+  for (int k = 0; k < kRowsPerLane; ++k) {
+    const int row = row0 + k * RPC;
+    float m = absmax_value<InT>(absmax_acc<InT>(0u, u[k]));
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int e = pow2_exponent(m, 40);
+    const float sc = pow2f(e);
+    const InT* xe = reinterpret_cast<const InT*>(&u[k]);
+    uint32_t q[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      q[i] = __float_as_uint(fminf(fmaxf(__fmaf_rn(to_f32(xe[i]), sc, 12582912.0f), 12582912.0f - 127.0f), 12582912.0f + 127.0f));
+    if (row < rows) {
+      int8_t* dst = q8 + (long long)row * DH + sub * N;
+      if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(pack4_s8(q[0], q[1], q[2], q[3]), pack4_s8(q[4], q[5], q[6], q[7]));
+      else *reinterpret_cast<uint32_t*>(dst) = pack4_s8(q[0], q[1], q[2], q[3]);
+      if (sub == 0) eq[row] = e;
+    }
+  }
+}
+
+template <typename Plan, typename InT, int DH>
+__global__ void __launch_bounds__(kStepPlanThreads)
+step_plan_quant_kernel(const Plan plan, const InT* __restrict__ x, Strides4 xs, int N, int H, int8_t* __restrict__ q8,
+                       int32_t* __restrict__ eq) {
+  pdl_launch_dependents();                       // the attention kernel may start its setup
+  if (blockIdx.x == 0) step_plan(plan);
+  else quant_tokens<InT, DH>((int)blockIdx.x - 1, x, xs, N * H, H, q8, eq);
 }
 
 }  // namespace lssab8

@@ -359,12 +359,70 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   pdl_wait();                                        // the quantisers' lattice is complete
+  if constexpr (SRC == kSrcShared) pdl_launch_dependents();   // the batch's own blocks may run beside this kernel
   if constexpr (PAGED) {
     nitems = pf_paged_items<SRC>(p);
     nrounds = (nitems + (int)gridDim.x - 1) / (int)gridDim.x;
   }
 
-  if (warp == 0) {
+  if (PAGED && warp == 0) {
+    // ================================================================ TMA producer, paged
+    // Lane 0 waits and posts the byte counts; lane i < 8 holds page i of a block (loaded a block ahead) and
+    // issues its key box and value page, so a block's 16 copies are two issues of the warp.
+    constexpr uint32_t kPage = 16 * DH;
+    int jj = 0, tt = 0;
+    bool ok = true;
+    PfItem it;
+    for (int rd = 0; ok && rd < nrounds; ++rd) {
+      if (!next_item(rd, it)) continue;
+      const int qb = tt & 1;
+      const int32_t* bt = p.pg.block_table + (long long)it.b * p.pg.max_pages;
+      const int npages = (it.T + 15) / 16;
+      auto page_of = [&](int j) -> int {
+        const int i = (it.j0 + j) * 8 + lane;
+        return lane < 8 && i < npages ? bt[i] : 0;
+      };
+      int pg = page_of(0);
+      if (lane == 0) {
+        ok = mbar_wait(&bars[kBarQEmpty + qb], ((tt >> 1) & 1) ^ 1, abort_flag, p.err, 128, p.wait_ns);
+        if (ok) {
+          if constexpr (SRC == kSrcRows) {
+            mbar_expect_tx(&bars[kBarQFull + qb], L::kTile);
+            tma_load_3d(smem + L::kQ + qb * L::kTile, &tm_q, 0, it.h, it.row0, &bars[kBarQFull + qb]);
+          } else {
+            mbar_expect_tx(&bars[kBarQFull + qb], (uint32_t)(p.pg.seqs_per_tile * p.group * DH));
+            tma_load_3d(smem + L::kQ + qb * L::kTile, &tm_q, 0, it.g * p.group, it.tile * p.pg.seqs_per_tile,
+                        &bars[kBarQFull + qb]);
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      for (int j = 0; ok && j < it.nb; ++j, ++jj) {
+        const int s = jj & 1;
+        const uint32_t ph = (jj >> 1) & 1;
+        const int npg = min(8, npages - (it.j0 + j) * 8);
+        if (lane < npg && (pg < 0 || pg >= p.pg.num_pages)) { atomicOr(p.err, kDevBadPage); pg = 0; }
+        const long long row = (long long)pg * p.KVH + it.g;
+        const int next = j + 1 < it.nb ? page_of(j + 1) : 0;
+        if (lane == 0) {
+          ok = mbar_wait(&bars[kBarKEmpty + s], ph ^ 1, abort_flag, p.err, 128, p.wait_ns);
+          if (ok) mbar_expect_tx(&bars[kBarKFull + s], npg * kPage);
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        if (ok && lane < npg)
+          tma_load_2d(smem + L::kK + s * L::kTile + lane * kPage, &tm_k, 0, (int)(row * 16), &bars[kBarKFull + s]);
+        if (ok && lane == 0) {
+          ok = mbar_wait(&bars[kBarVEmpty + s], ph ^ 1, abort_flag, p.err, 128, p.wait_ns);
+          if (ok) mbar_expect_tx(&bars[kBarVFull + s], npg * kPage);
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        if (ok && lane < npg)
+          bulk_g2s(smem + L::kV + s * L::kTile + lane * kPage, p.pg.v8p + row * kPage, kPage, &bars[kBarVFull + s]);
+        pg = next;
+      }
+      ++tt;
+    }
+  } else if (warp == 0) {
     // ================================================================ TMA producer
     if (lane == 0) {
       int jj = 0, tt = 0;
@@ -378,46 +436,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const int qb = tt & 1;
         // buffer qb is free once item tt - 2's last QK has finished and its workers are done
         if (!mbar_wait(&bars[kBarQEmpty + qb], ((tt >> 1) & 1) ^ 1, abort_flag, p.err, 128, p.wait_ns)) { ok = false; break; }
-        if constexpr (PAGED) {
-          constexpr uint32_t kPage = 16 * DH;
-          if constexpr (SRC == kSrcRows) {
-            mbar_expect_tx(&bars[kBarQFull + qb], L::kTile);
-            tma_load_2d(smem + L::kQ + qb * L::kTile, &tm_q, 0, it.h * p.Tpad + it.row0, &bars[kBarQFull + qb]);
-          } else {
-            mbar_expect_tx(&bars[kBarQFull + qb], (uint32_t)(p.pg.seqs_per_tile * p.group * DH));
-            tma_load_3d(smem + L::kQ + qb * L::kTile, &tm_q, 0, it.g * p.group, it.tile * p.pg.seqs_per_tile,
-                        &bars[kBarQFull + qb]);
-          }
-          const int32_t* bt = p.pg.block_table + (long long)it.b * p.pg.max_pages;
-          const int npages = (it.T + 15) / 16;
-          for (int j = 0; j < it.nb; ++j, ++jj) {
-            const int s = jj & 1;
-            const uint32_t ph = (jj >> 1) & 1;
-            const int p0 = (it.j0 + j) * 8;
-            const int npg = min(8, npages - p0);
-            long long pr[8];                             // page rows, in flight during the wait
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pr[i] = i < npg ? bt[p0 + i] : 0;
-            if (!mbar_wait(&bars[kBarKEmpty + s], ph ^ 1, abort_flag, p.err, 128, p.wait_ns)) { ok = false; break; }
-            mbar_expect_tx(&bars[kBarKFull + s], npg * kPage);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (i >= npg) break;
-              if (pr[i] < 0 || pr[i] >= p.pg.num_pages) { atomicOr(p.err, kDevBadPage); pr[i] = 0; }
-              pr[i] = pr[i] * p.KVH + it.g;
-              tma_load_2d(smem + L::kK + s * L::kTile + i * kPage, &tm_k, 0, (int)(pr[i] * 16), &bars[kBarKFull + s]);
-            }
-            if (!mbar_wait(&bars[kBarVEmpty + s], ph ^ 1, abort_flag, p.err, 128, p.wait_ns)) { ok = false; break; }
-            mbar_expect_tx(&bars[kBarVFull + s], npg * kPage);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (i >= npg) break;
-              bulk_g2s(smem + L::kV + s * L::kTile + i * kPage, p.pg.v8p + pr[i] * kPage, kPage, &bars[kBarVFull + s]);
-            }
-          }
-          ++tt;
-          continue;
-        }
         mbar_expect_tx(&bars[kBarQFull + qb], L::kTile + (SINK ? DH : 0));
         tma_load_2d(smem + L::kQ + qb * L::kTile, &tm_q, 0, qrow0, &bars[kBarQFull + qb]);
         if (SINK) bulk_g2s(v0row + qb * 128, p.v8 + (long long)krow0 * DH, DH, &bars[kBarQFull + qb]);
@@ -552,7 +570,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int32_t *ekg, *evg;
       if constexpr (PAGED) {
         if constexpr (SRC == kSrcRows) {
-          eqr = p.eq[(long long)h * p.Tpad + it.row0 + r];
+          eqr = it.row0 + r < p.Tpad ? p.eq[(long long)(it.row0 + r) * p.H + h] : 0;   // [N, H], Tpad = N
         } else {
           const int sq = r / p.group, seq = tile * p.pg.seqs_per_tile + sq;
           srow = (sq < p.pg.seqs_per_tile && seq < p.B) ? seq * p.H + g * p.group + (r - sq * p.group) : -1;
@@ -713,31 +731,49 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         return true;
       };
 
-      // kSrcShared, an item of a few blocks: the exact partials of block jf, as the decode stores them
+      // kSrcShared, an item of a few blocks: the exact partials of block jf, as the decode stores them.  A lane
+      // holds 16 channels of one row, so a warp's 32 row pieces of 64 bytes go through its 2 KB of shared
+      // memory (16-byte chunks XOR-swizzled, no bank conflicts) and leave as whole sectors, 8 pieces an
+      // instruction.  Stored straight from the registers, 32 rows an instruction, a block took 5.1 us, staged
+      // 3.3 us (folding it takes 2.1 us).
+      long long mine = -1, prow_of[4];                      // this row; rows of the pieces this lane stores: 8 i + lane / 4
+      if constexpr (SRC == kSrcShared) {
+        const int seq = srow / p.H, hh = srow - seq * p.H - g * p.group;
+        if (srow >= 0) mine = (((long long)seq * p.KVH + g) * p.pg.max_part + it.j0 - p.pg.nfold * kSEG) * p.group + hh;
+  #pragma unroll
+        for (int i = 0; i < 4; ++i) prow_of[i] = __shfl_sync(0xffffffffu, mine, (8 * i + (lane >> 2)) & 15);
+      }
       auto store_partials = [&](int jf, int nbb, int lbt, int eh0v) -> bool {
         const int jgf = jj0 + jf;
         const int sa = jgf & 1;
         if (!warp_poll(&bars[kBarAFull + sa], (uint32_t)((jgf >> 1) & 1), abort_flag, p.err, p.wait_ns)) return false;
         tc_fence_after();
         const uint32_t abase = rowt + kColA + sa * 128;
-        const int seq = srow / p.H, hh = srow - seq * p.H - g * p.group;
-        const long long row = (((long long)seq * p.KVH + g) * p.pg.max_part + it.j0 + jf - p.pg.nfold * kSEG) * p.group + hh;
+        const uint32_t stage = smem_u32(smem + L::kBytes) + (warp - 2) * 2048;
   #pragma unroll
         for (int cc = 0; cc < HALF / 16; ++cc) {
           uint32_t a[16];
           tmem_ld16x2<HALF>(abase + cc * 16, a);
           tc_wait_ld();
-          if (srow >= 0) {
-            int4* dst = reinterpret_cast<int4*>(p.pg.partA + row * DH + kh * HALF + cc * 16);
+          __syncwarp();                                  // the pieces of the last pass have left
   #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              __stcg(dst + c, make_int4((int)(a[4 * c] - kMagicBits), (int)(a[4 * c + 1] - kMagicBits),
-                                        (int)(a[4 * c + 2] - kMagicBits), (int)(a[4 * c + 3] - kMagicBits)));
+          for (int c = 0; c < 4; ++c)
+            st_shared_v4(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), a[4 * c] - kMagicBits, a[4 * c + 1] - kMagicBits,
+                         a[4 * c + 2] - kMagicBits, a[4 * c + 3] - kMagicBits);
+          __syncwarp();
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int piece = 8 * i + (lane >> 2), c = lane & 3;   // piece = 16 half + row
+            const uint4 v = ld_shared_v4(stage + piece * 64 + ((c ^ ((piece >> 1) & 3)) << 4));
+            if (prow_of[i] >= 0)
+              __stcg(reinterpret_cast<uint4*>(p.pg.partA + (prow_of[i] + (long long)jf * p.group) * DH + (piece >> 4) * HALF +
+                                              cc * 16 + c * 4), v);
           }
         }
         tc_fence_before();
         mbar_arrive(&bars[kBarAEmpty + sa]);
-        if (srow >= 0 && kh == 0) __stcg(p.pg.partM + row, make_int4(nbb, lbt, sink0 && jf == 0 ? eh0v : 0, 0));
+        if (mine >= 0 && kh == 0)
+          __stcg(p.pg.partM + mine + (long long)jf * p.group, make_int4(nbb, lbt, sink0 && jf == 0 ? eh0v : 0, 0));
         return true;
       };
       auto finish_block = [&](int jf, int nbb, int lbt, int evj, int eh0v, bool live) -> bool {

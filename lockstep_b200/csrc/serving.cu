@@ -1,5 +1,6 @@
 // C ABI of the serving-step operators (declarations: include/lssab8.h): rotary positions, step tables,
 // packed prompt rows over the paged lattice, and decode over a shared prefix.
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/lssab8.h"
@@ -15,22 +16,29 @@ using namespace lssab8;
 
 namespace {
 
+// A kernel's shared-memory limit, raised once on each device (the runtime call costs 1 us a launch).
+struct SmemAttr {
+  std::atomic<uint64_t> done{0};
+  template <typename K> bool set(K kfn, int smem) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (done.load(std::memory_order_acquire) >> dev & 1) return true;
+    if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
+    done.fetch_or(1ull << dev, std::memory_order_release);
+    return true;
+  }
+};
+
 // ------------------------------------------------------------------ rotary
 bool rot_args_ok(const void* freq, int rot, int dh, int layout) {
   return freq && dh > 0 && dh <= kRotMaxDim && rot > 0 && rot <= dh && rot % 2 == 0 &&
          (layout == kRotHalf || layout == kRotInterleaved);
 }
 
-// Tokens a CTA and heads a CTA: a table of at most 16 KB, then enough CTAs for two an SM before a CTA
-// takes more rows (small steps are latency: one token a CTA, its heads split).
-void rot_shape(long long tokens, int heads, int rot, int sms, int* tpc, int* hpc) {
-  const long long want = 2LL * sms;
-  int t = std::max(1, std::min(16, 16384 / (rot * 4)));
-  while (t > 1 && (tokens + t - 1) / t < want) t >>= 1;
-  *tpc = t;
-  const long long ctas = (tokens + t - 1) / t;
-  const long long split = std::max<long long>(1, std::min<long long>(heads, want / std::max<long long>(ctas, 1)));
-  *hpc = (int)((heads + split - 1) / split);
+// Warps a token: one, or for few tokens as many as give every SM two CTAs, down to four heads a warp.
+int rot_chunks(long long tokens, int heads, int sms) {
+  const long long want = 2LL * sms * kRotWarps;
+  return (int)std::max<long long>(1, std::min<long long>((heads + 3) / 4, want / tokens));
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -38,29 +46,74 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 template <typename T, int VEC>
 int launch_rotate(const void* x, const int64_t* xs, void* y, const int64_t* ys, int B, int H, int T_, const RotPlan& pl,
                   const RotPos& pos, int sms, cudaStream_t st) {
-  int tpc, hpc;
-  rot_shape((long long)B * T_, H, pl.rot, sms, &tpc, &hpc);
-  const long long tiles = (long long)B * ((T_ + tpc - 1) / tpc);
-  const int hs = (H + hpc - 1) / hpc;
-  if (tiles > 0x7FFFFFFF || hs > 65535) return kErrArg;
-  auto kfn = pl.layout == kRotHalf ? rotate_kernel<T, VEC, kRotHalf> : rotate_kernel<T, VEC, kRotInterleaved>;
-  kfn<<<dim3((unsigned)tiles, hs), kRotThreads, tpc * pl.rot * 4, st>>>(
-      static_cast<const T*>(x), xs[0], xs[1], xs[2], xs[3], static_cast<T*>(y), ys[0], ys[1], ys[2], ys[3], H, T_, tpc,
-      hpc, pl, pos);
+  const long long tokens = (long long)B * T_;
+  const int chunks = rot_chunks(tokens, H, sms);
+  const long long grid = (tokens * chunks + kRotWarps - 1) / kRotWarps;
+  if (grid > 0x7FFFFFFF) return kErrArg;
+  const bool full = pl.rot == pl.dh && VEC > 1;
+  auto kfn = pl.layout == kRotHalf ? (full ? rotate_kernel<T, VEC, kRotHalf, true> : rotate_kernel<T, VEC, kRotHalf, false>)
+                                   : (full ? rotate_kernel<T, VEC, kRotInterleaved, true>
+                                           : rotate_kernel<T, VEC, kRotInterleaved, false>);
+  kfn<<<(unsigned)grid, 32 * kRotWarps, kRotWarps * pl.rot * 4, st>>>(
+      static_cast<const T*>(x), xs[0], xs[1], xs[2], xs[3], static_cast<T*>(y), ys[0], ys[1], ys[2], ys[3], B, H, T_, chunks,
+      pl, pos);
   return launch_rc();
 }
 
 template <typename T, typename C, int VEC>
 int launch_append(const RotAppend& a, const RotPlan& pl, const RotPos& pos, const DevState* ds, cudaStream_t st) {
-  int tpc, hpc;
-  const int heads = a.H + 2 * a.KVH;
-  rot_shape(a.N, heads, pl.rot, ds->num_sms, &tpc, &hpc);
-  const int hs = (heads + hpc - 1) / hpc;
-  if (hs > 65535) return kErrArg;
-  auto kfn = pl.layout == kRotHalf ? rotate_append_kernel<T, C, VEC, kRotHalf>
-                                   : rotate_append_kernel<T, C, VEC, kRotInterleaved>;
-  kfn<<<dim3((a.N + tpc - 1) / tpc, hs), kRotThreads, tpc * pl.rot * 4, st>>>(a, tpc, hpc, pl, pos, ds->err);
+  const int chunks = rot_chunks(a.N, a.H, ds->num_sms), kv_chunks = std::min(chunks, (a.KVH + 3) / 4);
+  const long long grid = ((long long)a.N * chunks + kRotWarps - 1) / kRotWarps;
+  if (grid > 0x7FFFFFFF) return kErrArg;
+  const bool full = pl.rot == pl.dh && VEC > 1;
+  auto kfn = pl.layout == kRotHalf ? (full ? rotate_append_kernel<T, C, VEC, kRotHalf, true>
+                                           : rotate_append_kernel<T, C, VEC, kRotHalf, false>)
+                                   : (full ? rotate_append_kernel<T, C, VEC, kRotInterleaved, true>
+                                           : rotate_append_kernel<T, C, VEC, kRotInterleaved, false>);
+  kfn<<<dim3((unsigned)grid, 3), 32 * kRotWarps, kRotWarps * pl.rot * 4, st>>>(a, chunks, kv_chunks, pl, pos, ds->err);
   return launch_rc();
+}
+
+// ------------------------------------------------------------------ plans
+// The call's plan and the quantiser of its queries [N, H, dh] -> q8 [N, H, dh], eq [N, H], in one launch when the
+// rows are 16-byte vectors.
+template <typename Plan>
+int plan_and_quant(const Plan& plan, const void* q, int dtype, int N, int H, int dh, const int64_t* qs, int8_t* q8,
+                   int32_t* eq, cudaStream_t st) {
+  return with_in_dtype(dtype, [&](auto tag) -> int {
+    using InT = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
+    const Strides4 s{0, qs[0], qs[1], qs[2]};                  // "heads" are tokens, "rows" the token's heads
+    if (!vec_ok<InT>(q, s, dh)) {
+      step_plan_kernel<Plan><<<1, kStepPlanThreads, 0, st>>>(plan);
+      const int rc = launch_rc();
+      const int64_t q4[4] = {0, qs[0], qs[1], qs[2]};
+      return rc ? rc : lssab8_quant_rows(q, dtype, 1, N, H, dh, q4, H, q8, eq, st);
+    }
+    const int rpw = 32 / (dh / Vec16<InT>::kN);
+    const long long per_cta = 8LL * rpw * kRowsPerLane;
+    const long long ctas = ((long long)N * H + per_cta - 1) / per_cta;
+    if (dh == 128)
+      step_plan_quant_kernel<Plan, InT, 128><<<(unsigned)(ctas + 1), kStepPlanThreads, 0, st>>>(
+          plan, static_cast<const InT*>(q), s, N, H, q8, eq);
+    else
+      step_plan_quant_kernel<Plan, InT, 64><<<(unsigned)(ctas + 1), kStepPlanThreads, 0, st>>>(
+          plan, static_cast<const InT*>(q), s, N, H, q8, eq);
+    return launch_rc();
+  });
+}
+
+// q8 [B, H, dh] as boxes of (dh, the kv head's group, sequences): a tile's rows in (sequence, head) order
+int make_tmap_group(CUtensorMap* tm, const void* base, int B, int H, int dh, int group, int seqs) {
+  const auto encode = encode_fn();
+  if (!encode) return kErrCuda;
+  cuuint64_t dims[3] = {(cuuint64_t)dh, (cuuint64_t)H, (cuuint64_t)B};
+  cuuint64_t strides[2] = {(cuuint64_t)dh, (cuuint64_t)H * dh};
+  cuuint32_t box[3] = {(cuuint32_t)dh, (cuuint32_t)group, (cuuint32_t)seqs};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, dh == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? kOk : kErrCuda;
 }
 
 // ------------------------------------------------------------------ packed prompt rows
@@ -68,14 +121,11 @@ struct RowsWs {
   size_t q8, eq, tile_off, tiles, ntiles, total;
 };
 
-inline int rows_pitch(int N) { return tpad_of(N) + 128; }     // a tile may start at any row below N
-
 RowsWs rows_ws(int N, int H, int dh, int B) {
   RowsWs w{};
-  const size_t pitch = (size_t)rows_pitch(N);
   size_t o = 0;
-  w.q8 = o; o += align256((size_t)H * pitch * dh);
-  w.eq = o; o += align256((size_t)H * pitch * 4);
+  w.q8 = o; o += align256((size_t)N * H * dh);
+  w.eq = o; o += align256((size_t)N * H * 4);
   w.tile_off = o; o += align256((size_t)(B + 1) * 4);
   w.tiles = o; o += align256(((size_t)N / 128 + B) * 16);
   w.ntiles = o; o += 256;
@@ -86,10 +136,11 @@ RowsWs rows_ws(int N, int H, int dh, int B) {
 template <int DH, bool SINK, typename OutT, bool MULTI, int SRC>
 int launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tk, const PrefillArgs& a, long long items, int num_sms,
                    cudaStream_t st) {
-  int smem = kTabBytes + 1024 + PrefillSmem<DH>::kBytes;
+  int smem = kTabBytes + 1024 + PrefillSmem<DH>::kBytes + (SRC == kSrcShared ? 8 * 2048 : 0);   // (the partials' stage)
   if (smem < 116 * 1024) smem = 116 * 1024;                   // one CTA (one 512-column TMEM allocation) an SM
   auto kfn = prefill_kernel<DH, SINK, OutT, MULTI, false, false, SRC>;
-  if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kErrCuda;
+  static SmemAttr attr;
+  if (!attr.set(kfn, smem)) return kErrCuda;
   const int grid = (int)std::min<long long>(items, (long long)std::max(num_sms, 1));
   return launch_pdl(kfn, dim3(grid), dim3(kPrefillThreads), smem, st, tq, tk, tk, a);
 }
@@ -121,20 +172,6 @@ void prefill_consts(PrefillArgs* a, int dh, int* err) {
 }
 
 // ------------------------------------------------------------------ shared prefix
-// q8 [B, H, dh] as boxes of (dh, the kv head's group, sequences): a tile's rows in (sequence, head) order
-int make_tmap_group(CUtensorMap* tm, const void* base, int B, int H, int dh, int group, int seqs) {
-  const auto encode = encode_fn();
-  if (!encode) return kErrCuda;
-  cuuint64_t dims[3] = {(cuuint64_t)dh, (cuuint64_t)H, (cuuint64_t)B};
-  cuuint64_t strides[2] = {(cuuint64_t)dh, (cuuint64_t)H * dh};
-  cuuint32_t box[3] = {(cuuint32_t)dh, (cuuint32_t)group, (cuuint32_t)seqs};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, dh == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? kOk : kErrCuda;
-}
-
 // How the shared blocks are cut into items.  Row tiles x kv heads is the work of one block; the items are
 // folded segments and, for the rest, chunks of exact partials.
 struct SharedShape {
@@ -145,11 +182,16 @@ SharedShape shared_shape(int B, int KVH, int group, int shared_blocks, int num_s
   s.seqs_per_tile = 128 / group;
   s.row_tiles = (B + s.seqs_per_tile - 1) / s.seqs_per_tile;
   const long long per_block = (long long)KVH * s.row_tiles;
-  s.nfold = 0;
+  // A folded segment is 32 blocks one after another on one SM (2 us a block); partials run on all SMs at once but
+  // cost 6.5 us a block and SM, refold included.  Measured (32 to 128 sequences, groups 4 and 8, prefixes 2,048 to
+  // 32,768; partials / folded): 1,024 block tiles 71 / 85 us, 2,048 113 / 87 us, 4,096 186 / 97 us.
+  const long long segs = per_block * (shared_blocks / kSEG);
+  const long long waves = (segs + num_sms - 1) / num_sms;
+  s.nfold = per_block * shared_blocks > waves * kSEG * num_sms * 5 / 16 ? shared_blocks / kSEG : 0;
   const int rest = shared_blocks - s.nfold * kSEG;
   if (rest > 0) {
     const long long slots = std::max<long long>(1, num_sms / per_block);   // items a (tile, kv head) in one wave
-    s.chunk = (int)((rest + slots - 1) / slots);
+    s.chunk = s.nfold ? 4 : (int)((rest + slots - 1) / slots);
     s.nchunks = (rest + s.chunk - 1) / s.chunk;
   }
   return s;
@@ -182,9 +224,10 @@ int launch_own_tc(const DecodeArgs& a, int num_sms, cudaStream_t st) {
   if ((rc = make_tmap(&tq, a.q8, (long long)a.B * a.H, 128, 16))) return rc;
   const int smem = DecTcSmem::kBytes + 1024;
   auto kfn = decode_tc_kernel<SINK, OutT, GQ, true>;
-  if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kErrCuda;
-  const long long chunks = ((long long)a.B * a.KVH * (a.max_blocks - a.skip_blocks) + kDecChunk - 1) / kDecChunk;
-  const int grid = (int)std::max<long long>(1, std::min<long long>(chunks, 2LL * std::max(num_sms, 1)));
+  static SmemAttr attr;
+  if (!attr.set(kfn, smem)) return kErrCuda;
+  const long long blocks = (long long)a.B * a.KVH * (a.max_blocks - a.skip_blocks);
+  const int grid = (int)std::max<long long>(1, std::min<long long>(blocks, 2LL * std::max(num_sms, 1)));
   return launch_pdl(kfn, dim3(grid), dim3(DecWorkers<GQ>::kThreads), smem, st, tk, tq, a);
 }
 
@@ -203,9 +246,10 @@ int launch_shared_t(const DecodeArgs& a, const PrefillArgs& pa, const SharedShap
     } else {
       const int smem = DecodeSmem<DH>::kBytes + 128;
       auto kfn = decode_kernel<DH, SINK, float, true>;
-      if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kErrCuda;
-      kfn<<<dim3((a.max_blocks - a.skip_blocks + a.split_blocks - 1) / a.split_blocks, a.KVH, a.B), 128, smem, st>>>(a);
-      rc = launch_rc();
+      static SmemAttr attr;
+      if (!attr.set(kfn, smem)) return kErrCuda;
+      rc = launch_pdl(kfn, dim3((a.max_blocks - a.skip_blocks + a.split_blocks - 1) / a.split_blocks, a.KVH, a.B),
+                      dim3(128), smem, st, a);
     }
     if (rc) return rc;
   }
@@ -334,7 +378,7 @@ int lssab8_prefill_paged(const void* q, int dtype, const int64_t* qs, int N, int
   if (!q || !cu_q || !seq_lens || !block_table || !k8p || !v8p || !ek || !ev || (sink && !ev0) || !out || !workspace ||
       !strides_ok(qs, 3) || !strides_ok(os, 3) || B <= 0 || !shape_ok(1, H, KVH, N, dh) || max_blocks <= 0 ||
       max_pages <= 0 || num_pages <= 0 || (long long)num_pages * KVH * 16 > 0x7FFFFFFFll ||
-      (long long)H * rows_pitch(N) > 0x7FFFFFFFll || ((long long)N / 128 + B) * H > 0x7FFFFFFFll)
+      (long long)H * N > 0x7FFFFFFFll || ((long long)N / 128 + B) * H > 0x7FFFFFFFll)
     return kErrArg;
   if (dh != 64 && dh != 128) return kErrUnsupported;
   const RowsWs w = rows_ws(N, H, dh, B);
@@ -344,22 +388,18 @@ int lssab8_prefill_paged(const void* q, int dtype, const int64_t* qs, int N, int
   if (rc) return rc;
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int pitch = rows_pitch(N);
   int8_t* q8 = reinterpret_cast<int8_t*>(base + w.q8);
   int32_t* eq = reinterpret_cast<int32_t*>(base + w.eq);
   int4* tiles = reinterpret_cast<int4*>(base + w.tiles);
   int* ntiles = reinterpret_cast<int*>(base + w.ntiles);
   const RowsPlanArgs pa{cu_q, seq_lens, prefix_lens, active, B, N, max_blocks, max_pages,
                         reinterpret_cast<int*>(base + w.tile_off), tiles, N / 128 + B, ntiles, ds->err};
-  rows_plan_kernel<<<1, kRowsPlanThreads, 0, st>>>(pa);
-  if ((rc = launch_rc())) return rc;
-  const int64_t q4[4] = {0, qs[1], qs[0], qs[2]};
-  if ((rc = lssab8_quant_rows(q, dtype, 1, H, N, dh, q4, pitch, q8, eq, stream))) return rc;
+  if ((rc = plan_and_quant(pa, q, dtype, N, H, dh, qs, q8, eq, st))) return rc;
   CUtensorMap tq, tk;
-  if ((rc = make_tmap(&tq, q8, (long long)H * pitch, dh))) return rc;
+  if ((rc = make_tmap_group(&tq, q8, N, H, dh, 1, 128))) return rc;
   if ((rc = make_tmap(&tk, k8p, (long long)num_pages * KVH * 16, dh, 16))) return rc;
   PrefillArgs a{};
-  a.B = B; a.H = H; a.KVH = KVH; a.T = 0; a.dh = dh; a.Tpad = pitch; a.group = H / KVH;
+  a.B = B; a.H = H; a.KVH = KVH; a.T = 0; a.dh = dh; a.Tpad = N; a.group = H / KVH;
   a.eq = eq; a.ek = ek; a.ev = ev; a.ev0 = sink ? ev0 : nullptr;
   a.out = out; a.os1 = os[0]; a.os2 = os[1]; a.os3 = os[2]; a.out_dtype = out_dtype;
   prefill_consts(&a, dh, ds->err);
@@ -428,11 +468,8 @@ int lssab8_decode_shared(const void* q, int dtype, const int64_t* qs, int B, int
   p.pg.max_part = a.max_part; p.pg.partA = a.partA; p.pg.partM = a.partM;
   p.pg.segO = reinterpret_cast<float*>(base + w.segO);
   p.pg.segM = reinterpret_cast<int2*>(base + w.segM);
-  decode_plan_kernel<true><<<1, kPlanThreads, 0, st>>>(seq_lens, B, max_blocks, max_pages, a.blk_off, a.order, nullptr, 0,
-                                                        ds->err, shared_blocks, leader);
-  if ((rc = launch_rc())) return rc;
-  const int64_t q4[4] = {qs[0], qs[1], 0, qs[2]};
-  if ((rc = quant_queries_pdl(q, dtype, B, H, dh, q4, q8, eq, st))) return rc;
+  const SharedPlanArgs plan{seq_lens, B, max_blocks, max_pages, a.blk_off, a.order, ds->err, shared_blocks, leader};
+  if ((rc = plan_and_quant(plan, q, dtype, B, H, dh, qs, q8, eq, st))) return rc;
   if (dh == 128) return sink ? launch_shared_out<128, true>(out_dtype, a, p, sh, ds->num_sms, st)
                              : launch_shared_out<128, false>(out_dtype, a, p, sh, ds->num_sms, st);
   return sink ? launch_shared_out<64, true>(out_dtype, a, p, sh, ds->num_sms, st)

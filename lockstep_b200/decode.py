@@ -253,7 +253,7 @@ def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtyp
     if active is not None and (tuple(active.shape) != (B,) or active.dtype != torch.bool):
         raise ValueError("active must be [%d] bool" % B)
     if out is None:
-        out = torch.empty((N, H, dh), dtype=out_dtype or q.dtype, device=dev)
+        out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
     _check_out(out, (N, H, dh), dev)
     if N == 0:
         return out
@@ -266,14 +266,14 @@ def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtyp
         raise ValueError("unsupported shape")
     # the workspace comes from torch's allocator on this stream at every call, so calls on other streams
     # and captured graphs never share one
-    with torch.cuda.device(dev):
+    with _A._on(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.check(L.lssab8_prefill_paged(
-            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64x(q.stride()), N, H, kv.KVH, dh, cu_q.data_ptr(),
+            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64c(q.stride()), N, H, kv.KVH, dh, cu_q.data_ptr(),
             kv.seq_lens.data_ptr(), None if prefix_lens is None else prefix_lens.data_ptr(),
             None if active is None else active.data_ptr(), B, kv.block_table.data_ptr(), kv.block_table.shape[1],
             kv.num_pages, kv.k8p.data_ptr(), kv.v8p.data_ptr(), kv.ek.data_ptr(), kv.ev.data_ptr(), kv.ev0.data_ptr(),
-            kv.max_blocks, int(kv.sink), out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64x(out.stride()),
+            kv.max_blocks, int(kv.sink), out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64c(out.stride()),
             ws.data_ptr(), nbytes, _A._stream_handle(dev)), "lssab8_prefill_paged")
     if check:
         _A.check_device_errors(dev)
@@ -301,19 +301,19 @@ def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
     if shared_len // KB > kv.max_blocks or shared_len // KB * (KB // PAGE) > kv.block_table.shape[1]:
         raise ValueError("the lattice holds at most %d blocks a sequence" % kv.max_blocks)
     if out is None:
-        out = torch.empty((B, H, dh), dtype=out_dtype or q.dtype, device=dev)
+        out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
     _check_out(out, (B, H, dh), dev)
     L = _lib.load()
-    with torch.cuda.device(dev):
+    with _A._on(dev):
         nbytes = L.lssab8_decode_shared_workspace_size(B, H, kv.KVH, dh, kv.max_blocks, shared_len)
         if nbytes == 0:
             raise ValueError("unsupported decode shape")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)       # a call's own, as in prefill_paged
         _lib.check(L.lssab8_decode_shared(
-            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64x(q.stride()), B, H, kv.KVH, dh, kv.seq_lens.data_ptr(),
+            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64c(q.stride()), B, H, kv.KVH, dh, kv.seq_lens.data_ptr(),
             shared_len, kv.block_table.data_ptr(), kv.block_table.shape[1], kv.num_pages, kv.k8p.data_ptr(),
             kv.v8p.data_ptr(), kv.ek.data_ptr(), kv.ev.data_ptr(), kv.ev0.data_ptr(), kv.max_blocks, int(kv.sink),
-            out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64x(out.stride()), ws.data_ptr(), nbytes,
+            out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64c(out.stride()), ws.data_ptr(), nbytes,
             _A._stream_handle(dev)), "lssab8_decode_shared")
     if check:
         _A.check_device_errors(dev)

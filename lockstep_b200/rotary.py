@@ -15,6 +15,7 @@ theta_i = base^(-2 i / rotary_dim) for pair i, scaled for long contexts by one o
 The angle of position p is p theta_i, kept as an exact fraction of a turn (64-bit integer arithmetic), so it
 is as good at position 10^6 as at 1.
 """
+import functools
 import math
 from dataclasses import dataclass
 
@@ -81,15 +82,19 @@ def _check_positions(positions):
         raise TypeError("positions must be int32 or int64, got %s" % positions.dtype)
 
 
-def _written_once(t):
-    """No two elements of t share memory (as far as strides tell)."""
-    dims = sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1)
+@functools.lru_cache(maxsize=4096)
+def _apart(strides, shape):
     end = 0
-    for st, n in dims:
+    for st, n in sorted((st, n) for st, n in zip(strides, shape) if n > 1):
         if st <= end:
             return False
         end += st * (n - 1)
     return True
+
+
+def _written_once(t):
+    """No two elements of t share memory (as far as strides tell)."""
+    return _apart(t.stride(), t.shape)
 
 
 def _launch(x, positions, plan, inverse, out):
@@ -99,11 +104,11 @@ def _launch(x, positions, plan, inverse, out):
     x4, y4 = (x, out) if x.dim() == 4 else (x.transpose(0, 1)[None], out.transpose(0, 1)[None])
     B, H, T, dh = x4.shape
     ps = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
-    with torch.cuda.device(dev):
+    with _A._on(dev):
         _lib.check(_lib.load().lssab8_rotate(
-            x4.data_ptr(), _A.dtype_code(x.dtype), B, H, T, dh, _lib.i64x(x4.stride()), positions.data_ptr(),
-            int(positions.dtype == torch.int64), _lib.i64x(ps), plan.freq.data_ptr(), plan.factor, plan.rotary_dim,
-            _LAYOUTS[plan.layout], int(bool(inverse)), y4.data_ptr(), _lib.i64x(y4.stride()), _A._stream_handle(dev)),
+            x4.data_ptr(), _A.dtype_code(x.dtype), B, H, T, dh, _lib.i64c(x4.stride()), positions.data_ptr(),
+            int(positions.dtype == torch.int64), _lib.i64c(ps), plan.freq.data_ptr(), plan.factor, plan.rotary_dim,
+            _LAYOUTS[plan.layout], int(bool(inverse)), y4.data_ptr(), _lib.i64c(y4.stride()), _A._stream_handle(dev)),
             "lssab8_rotate")
     return out
 
@@ -170,7 +175,7 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         raise ValueError("rotate_append has no gradient (use rotate)")
     if out is None:
-        out = torch.empty((N, H, dh), dtype=query.dtype, device=dev)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev:
         raise ValueError("out must have the query's shape, dtype and device")
     for t in (query, key, value, k_cache, v_cache, out):
@@ -182,14 +187,14 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
     if N == 0:
         return out
     slot_mapping = slot_mapping.contiguous()
-    with torch.cuda.device(dev):
+    with _A._on(dev):
         _lib.check(_lib.load().lssab8_rotate_append(
             query.data_ptr(), key.data_ptr(), value.data_ptr(), _A.dtype_code(query.dtype), N, H, KVH, dh,
-            _lib.i64x(query.stride()[:2]), _lib.i64x(key.stride()[:2]), _lib.i64x(value.stride()[:2]),
+            _lib.i64c(query.stride()[:2]), _lib.i64c(key.stride()[:2]), _lib.i64c(value.stride()[:2]),
             positions.data_ptr(), int(positions.dtype == torch.int64), positions.stride(0), plan.freq.data_ptr(),
-            plan.factor, plan.rotary_dim, _LAYOUTS[plan.layout], out.data_ptr(), _lib.i64x(out.stride()[:2]),
-            k_cache.data_ptr(), v_cache.data_ptr(), _A.dtype_code(k_cache.dtype), _lib.i64x(k_cache.stride()[:3]),
-            _lib.i64x(v_cache.stride()[:3]), k_cache.shape[0], slot_mapping.data_ptr(), _A._stream_handle(dev)),
+            plan.factor, plan.rotary_dim, _LAYOUTS[plan.layout], out.data_ptr(), _lib.i64c(out.stride()[:2]),
+            k_cache.data_ptr(), v_cache.data_ptr(), _A.dtype_code(k_cache.dtype), _lib.i64c(k_cache.stride()[:3]),
+            _lib.i64c(v_cache.stride()[:3]), k_cache.shape[0], slot_mapping.data_ptr(), _A._stream_handle(dev)),
             "lssab8_rotate_append")
     if check:
         _A.check_device_errors(dev)
