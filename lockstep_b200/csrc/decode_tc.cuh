@@ -258,9 +258,7 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();                             // the refold kernel may queue up behind us
-  // the plan and the query quantiser are complete.  (SHARED: the shared-prefix kernel before this one let it
-  // start after its own wait for them; it does not read that kernel's output and runs beside it.)
-  if (!SHARED) pdl_wait();
+  pdl_wait();                                          // the plan and the query quantiser are complete
 
   if (warp == 0) {
     // ================================================================ TMA producer
@@ -486,7 +484,6 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   }
 
   // ---- teardown
-  if (SHARED) pdl_wait();                              // this grid completes after the shared-prefix kernel, so the refold's wait covers both
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

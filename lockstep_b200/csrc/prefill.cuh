@@ -359,7 +359,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   pdl_wait();                                        // the quantisers' lattice is complete
-  if constexpr (SRC == kSrcShared) pdl_launch_dependents();   // the batch's own blocks may run beside this kernel
+  // the kernel of the batch's own blocks may start: its setup (dh 128), all of it (dh 64), runs beside this one
+  if constexpr (SRC == kSrcShared) pdl_launch_dependents();
   if constexpr (PAGED) {
     nitems = pf_paged_items<SRC>(p);
     nrounds = (nitems + (int)gridDim.x - 1) / (int)gridDim.x;

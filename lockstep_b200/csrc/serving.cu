@@ -253,7 +253,10 @@ int launch_shared_t(const DecodeArgs& a, const PrefillArgs& pa, const SharedShap
     }
     if (rc) return rc;
   }
-  return launch_pdl(decode_merge_kernel<SINK, OutT, DH, true>, dim3(a.group, a.KVH, a.B), dim3(kMergeThreads), 0, st, a);
+  // (an ordinary launch: its waiting CTAs, started early, cost the kernels before it more than they save; 32 sequences
+  // on 8,192 tokens 48.5 -> 45.3 us)
+  decode_merge_kernel<SINK, OutT, DH, true><<<dim3(a.group, a.KVH, a.B), kMergeThreads, 0, st>>>(a);
+  return launch_rc();
 }
 
 template <int DH, bool SINK>

@@ -213,19 +213,24 @@ def decode(q, kv, split_blocks=4, out=None, out_dtype=None, check=True):
 
 
 def _check_lattice(q, kv, B, H, dh):
-    dev = _A._require_cuda(q, kv.k8p, kv.seq_lens, kv.block_table, kv.ek, kv.ev)
-    if dh != kv.dh or kv.seq_lens.numel() != B or kv.block_table.shape[0] != B or H % kv.KVH:
+    """Checks q [.., H, dh] against the lattice; returns (device, KVH)."""
+    k8p, lens, table, ek, ev, ev0 = kv.k8p, kv.seq_lens, kv.block_table, kv.ek, kv.ev, kv.ev0
+    dev = _A._require_cuda(q, k8p, kv.v8p, lens, table, ek, ev, ev0)
+    pages, KVH, _, lat_dh = k8p.shape
+    if (dh != lat_dh or H % KVH or lens.shape != (B,) or table.dim() != 2 or table.shape[0] != B or
+            ek.shape != (B, KVH, kv.max_blocks) or ev.shape != ek.shape or ev0.shape != (B, KVH) or pages < kv.num_pages):
         raise ValueError("query does not match the lattice")
-    if not (kv.seq_lens.is_contiguous() and kv.block_table.is_contiguous() and kv.ek.is_contiguous() and
-            kv.ev.is_contiguous() and kv.ev0.is_contiguous()):
-        raise ValueError("the lattice's lengths, table and exponents must be contiguous")
-    if kv.seq_lens.dtype != torch.int32 or kv.block_table.dtype != torch.int32:
-        raise TypeError("the lattice's lengths and table must be int32")
-    return dev
+    if not (lens.is_contiguous() and table.is_contiguous() and ek.is_contiguous() and ev.is_contiguous() and
+            ev0.is_contiguous() and k8p.is_contiguous() and kv.v8p.is_contiguous()):
+        raise ValueError("the lattice's pages, lengths, table and exponents must be contiguous")
+    i32 = torch.int32
+    if lens.dtype != i32 or table.dtype != i32 or ek.dtype != i32 or ev.dtype != i32 or ev0.dtype != i32:
+        raise TypeError("the lattice's lengths, table and exponents must be int32")
+    return dev, KVH
 
 
 def _check_out(out, shape, dev):
-    if tuple(out.shape) != tuple(shape) or out.device != dev:
+    if out.shape != shape or out.device != dev:
         raise ValueError("out must be %s on the query's device" % (tuple(shape),))
 
 
@@ -244,24 +249,25 @@ def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtyp
         raise ValueError("q must be [N, H, dh]")
     N, H, dh = q.shape
     B = kv.seq_lens.numel()
-    dev = _check_lattice(q, kv, B, H, dh)
+    dev, KVH = _check_lattice(q, kv, B, H, dh)
     _A._require_cuda(q, cu_q, *[t for t in (prefix_lens, active) if t is not None])
-    if tuple(cu_q.shape) != (B + 1,) or cu_q.dtype != torch.int32:
+    if cu_q.shape != (B + 1,) or cu_q.dtype != torch.int32:
         raise ValueError("cu_q must be [%d] int32" % (B + 1))
-    if prefix_lens is not None and (tuple(prefix_lens.shape) != (B,) or prefix_lens.dtype != torch.int32):
+    if prefix_lens is not None and (prefix_lens.shape != (B,) or prefix_lens.dtype != torch.int32):
         raise ValueError("prefix_lens must be [%d] int32" % B)
-    if active is not None and (tuple(active.shape) != (B,) or active.dtype != torch.bool):
+    if active is not None and (active.shape != (B,) or active.dtype != torch.bool):
         raise ValueError("active must be [%d] bool" % B)
     if out is None:
         out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
-    _check_out(out, (N, H, dh), dev)
+    else:
+        _check_out(out, q.shape, dev)
     if N == 0:
         return out
     cu_q = cu_q.contiguous()
     prefix_lens = None if prefix_lens is None else prefix_lens.contiguous()
     active = None if active is None else active.contiguous()
     L = _lib.load()
-    nbytes = L.lssab8_prefill_paged_workspace_size(N, H, kv.KVH, dh, B)
+    nbytes = L.lssab8_prefill_paged_workspace_size(N, H, KVH, dh, B)
     if nbytes == 0:
         raise ValueError("unsupported shape")
     # the workspace comes from torch's allocator on this stream at every call, so calls on other streams
@@ -269,7 +275,7 @@ def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtyp
     with _A._on(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.check(L.lssab8_prefill_paged(
-            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64c(q.stride()), N, H, kv.KVH, dh, cu_q.data_ptr(),
+            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64c(q.stride()), N, H, KVH, dh, cu_q.data_ptr(),
             kv.seq_lens.data_ptr(), None if prefix_lens is None else prefix_lens.data_ptr(),
             None if active is None else active.data_ptr(), B, kv.block_table.data_ptr(), kv.block_table.shape[1],
             kv.num_pages, kv.k8p.data_ptr(), kv.v8p.data_ptr(), kv.ek.data_ptr(), kv.ev.data_ptr(), kv.ev0.data_ptr(),
@@ -297,20 +303,21 @@ def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
         raise ValueError("shared_len must not be negative")
     if shared_len < KB:
         return decode(q, kv, out=out, out_dtype=out_dtype, check=check)
-    dev = _check_lattice(q, kv, B, H, dh)
+    dev, KVH = _check_lattice(q, kv, B, H, dh)
     if shared_len // KB > kv.max_blocks or shared_len // KB * (KB // PAGE) > kv.block_table.shape[1]:
         raise ValueError("the lattice holds at most %d blocks a sequence" % kv.max_blocks)
     if out is None:
         out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
-    _check_out(out, (B, H, dh), dev)
+    else:
+        _check_out(out, q.shape, dev)
     L = _lib.load()
     with _A._on(dev):
-        nbytes = L.lssab8_decode_shared_workspace_size(B, H, kv.KVH, dh, kv.max_blocks, shared_len)
+        nbytes = L.lssab8_decode_shared_workspace_size(B, H, KVH, dh, kv.max_blocks, shared_len)
         if nbytes == 0:
             raise ValueError("unsupported decode shape")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)       # a call's own, as in prefill_paged
         _lib.check(L.lssab8_decode_shared(
-            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64c(q.stride()), B, H, kv.KVH, dh, kv.seq_lens.data_ptr(),
+            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64c(q.stride()), B, H, KVH, dh, kv.seq_lens.data_ptr(),
             shared_len, kv.block_table.data_ptr(), kv.block_table.shape[1], kv.num_pages, kv.k8p.data_ptr(),
             kv.v8p.data_ptr(), kv.ek.data_ptr(), kv.ev.data_ptr(), kv.ev0.data_ptr(), kv.max_blocks, int(kv.sink),
             out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64c(out.stride()), ws.data_ptr(), nbytes,

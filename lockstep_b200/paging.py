@@ -28,10 +28,10 @@ class StepTables:
 
 def alloc_step_tables(n, cap, device):
     # two buffers, cut: a step's call pays for two allocations instead of six
-    qsl, lens, seq, used = torch.empty(2 * n + 2 + cap, dtype=torch.int32, device=device).split((n + 1, n, cap, 1))
-    slots, pos = torch.empty(2 * cap, dtype=torch.int64, device=device).split((cap, cap))
-    return StepTables(query_start_loc=qsl, seq_lens=lens, slot_mapping=slots, positions=pos, seq_index=seq,
-                      pages_used=used)
+    qsl, lens, seq, used = torch.unsafe_split_with_sizes(
+        torch.empty(2 * n + 2 + cap, dtype=torch.int32, device=device), (n + 1, n, cap, 1))
+    slots, pos = torch.empty((2, cap), dtype=torch.int64, device=device).unbind(0)
+    return StepTables(qsl, lens, slots, pos, seq, used)
 
 
 def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None, check=True):
@@ -43,16 +43,20 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
     Lengths that do not fit raise RuntimeError (device error 16) when checked."""
     dev = _A._require_cuda(lens, new_tokens, block_table, free_pages)
     n = lens.numel()
-    for t, name in ((lens, "lens"), (new_tokens, "new_tokens"), (block_table, "block_table"), (free_pages, "free_pages")):
-        if t.dtype != torch.int32:
-            raise TypeError("%s must be int32, got %s" % (name, t.dtype))
+    i32 = torch.int32
+    if lens.dtype != i32 or new_tokens.dtype != i32 or block_table.dtype != i32 or free_pages.dtype != i32:
+        raise TypeError("lens, new_tokens, block_table and free_pages must be int32")
     if lens.dim() != 1 or new_tokens.shape != lens.shape or not 0 < n <= MAX_SEQS:
         raise ValueError("lens and new_tokens must be [n], n from 1 to %d" % MAX_SEQS)
-    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] == 0 or free_pages.dim() != 1:
+    if block_table.dim() != 2 or free_pages.dim() != 1:
         raise ValueError("block_table must be [n, max_pages], free_pages [F]")
-    if block_table.stride(1) != 1 or block_table.stride(0) < block_table.shape[1]:
+    rows, width = block_table.shape
+    pitch, step = block_table.stride()
+    if rows != n or width == 0:
+        raise ValueError("block_table must be [n, max_pages], free_pages [F]")
+    if (step != 1 and width > 1) or (pitch < width and n > 1):
         raise ValueError("block_table rows must be contiguous and apart")
-    cap = int(max_tokens)
+    cap, nfree = int(max_tokens), free_pages.numel()
     if not 0 <= cap < 1 << 31:
         raise ValueError("max_tokens must be from 0 to 2^31 - 1")
     lens, new_tokens, free_pages = lens.contiguous(), new_tokens.contiguous(), free_pages.contiguous()
@@ -68,8 +72,8 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
             raise ValueError("out.seq_lens must not be the step's own lens or new_tokens")
     with _A._on(dev):
         _lib.check(_lib.load().lssab8_step_tables(
-            lens.data_ptr(), new_tokens.data_ptr(), n, block_table.data_ptr(), block_table.stride(0),
-            block_table.shape[1], free_pages.data_ptr() if free_pages.numel() else None, free_pages.numel(), cap,
+            lens.data_ptr(), new_tokens.data_ptr(), n, block_table.data_ptr(), max(pitch, width), width,
+            free_pages.data_ptr() if nfree else None, nfree, cap,
             out.query_start_loc.data_ptr(), out.seq_lens.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(),
             out.seq_index.data_ptr(), out.pages_used.data_ptr(), _A._stream_handle(dev)), "lssab8_step_tables")
     if check:

@@ -157,45 +157,57 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
     (any page, row and head strides; the cache's own dtype, one rounding) at slot_mapping [N] int64, page * 16 +
     row.  Slot -1 stores nothing.  Inference only: no gradient flows through it."""
     dev = _A._require_cuda(query, key, value, positions, slot_mapping, k_cache, v_cache, plan.freq)
-    if query.dim() != 3 or key.dim() != 3 or key.shape != value.shape or key.shape[0] != query.shape[0]:
-        raise ValueError("query must be [N, H, dh], key and value [N, KVH, dh]")
-    if not query.dtype == key.dtype == value.dtype or k_cache.dtype != v_cache.dtype:
-        raise TypeError("query, key and value must share one dtype, and so must the caches")
-    N, H, dh = query.shape
-    KVH = key.shape[1]
-    if dh != plan.head_dim or key.shape[2] != dh:
-        raise ValueError("the plan is for head dim %d" % plan.head_dim)
-    if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or tuple(k_cache.shape[1:]) != (PAGE, KVH, dh)):
-        raise ValueError("caches must be [num_pages, 16, %d, %d]" % (KVH, dh))
-    _check_positions(positions)
-    if tuple(positions.shape) != (N,) or tuple(slot_mapping.shape) != (N,):
-        raise ValueError("positions and slot_mapping must be [%d]" % N)
-    if slot_mapping.dtype != torch.int64:
-        raise TypeError("slot_mapping must be int64")
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+    if (query.requires_grad or key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
         raise ValueError("rotate_append has no gradient (use rotate)")
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev:
-        raise ValueError("out must have the query's shape, dtype and device")
-    for t in (query, key, value, k_cache, v_cache, out):
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
-            raise ValueError("channels must be contiguous")
-    for t in (out, k_cache, v_cache):
-        if not _written_once(t):
-            raise ValueError("out and the caches must not have elements that share memory")
-    if N == 0:
+    elif out.device != dev:
+        raise ValueError("out must be on the query's device")
+    args = _append_args(query.shape, query.stride(), query.dtype, key.shape, key.stride(), key.dtype, value.shape,
+                        value.stride(), value.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape,
+                        v_cache.stride(), v_cache.dtype, out.shape, out.stride(), out.dtype, positions.shape,
+                        positions.dtype, slot_mapping.shape, slot_mapping.dtype, plan.head_dim)
+    dims, qs, ks, vs, pos64, os_, cdt, kcs, vcs = args
+    if dims[1] == 0:
         return out
     slot_mapping = slot_mapping.contiguous()
     with _A._on(dev):
         _lib.check(_lib.load().lssab8_rotate_append(
-            query.data_ptr(), key.data_ptr(), value.data_ptr(), _A.dtype_code(query.dtype), N, H, KVH, dh,
-            _lib.i64c(query.stride()[:2]), _lib.i64c(key.stride()[:2]), _lib.i64c(value.stride()[:2]),
-            positions.data_ptr(), int(positions.dtype == torch.int64), positions.stride(0), plan.freq.data_ptr(),
-            plan.factor, plan.rotary_dim, _LAYOUTS[plan.layout], out.data_ptr(), _lib.i64c(out.stride()[:2]),
-            k_cache.data_ptr(), v_cache.data_ptr(), _A.dtype_code(k_cache.dtype), _lib.i64c(k_cache.stride()[:3]),
-            _lib.i64c(v_cache.stride()[:3]), k_cache.shape[0], slot_mapping.data_ptr(), _A._stream_handle(dev)),
-            "lssab8_rotate_append")
+            query.data_ptr(), key.data_ptr(), value.data_ptr(), *dims, qs, ks, vs, positions.data_ptr(), pos64,
+            positions.stride(0), plan.freq.data_ptr(), plan.factor, plan.rotary_dim, _LAYOUTS[plan.layout],
+            out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), cdt, kcs, vcs, k_cache.shape[0],
+            slot_mapping.data_ptr(), _A._stream_handle(dev)), "lssab8_rotate_append")
     if check:
         _A.check_device_errors(dev)
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _append_args(q, qst, qdt, k, kst, kdt, v, vst, vdt, kc, kcst, kcdt, vc, vcst, vcdt, o, ost, odt, pos, pdt, sl, sdt,
+                 head_dim):
+    """The checks of rotate_append's shapes, strides and types, and the arguments made from them; kept, since a
+    model's steps repeat them."""
+    if len(q) != 3 or len(k) != 3 or k != v or k[0] != q[0]:
+        raise ValueError("query must be [N, H, dh], key and value [N, KVH, dh]")
+    if not qdt == kdt == vdt or kcdt != vcdt:
+        raise TypeError("query, key and value must share one dtype, and so must the caches")
+    N, H, dh = q
+    KVH = k[1]
+    if dh != head_dim or k[2] != dh:
+        raise ValueError("the plan is for head dim %d" % head_dim)
+    if len(kc) != 4 or kc != vc or tuple(kc[1:]) != (PAGE, KVH, dh):
+        raise ValueError("caches must be [num_pages, 16, %d, %d]" % (KVH, dh))
+    if pdt not in (torch.int32, torch.int64):
+        raise TypeError("positions must be int32 or int64, got %s" % pdt)
+    if tuple(pos) != (N,) or tuple(sl) != (N,):
+        raise ValueError("positions and slot_mapping must be [%d]" % N)
+    if sdt != torch.int64:
+        raise TypeError("slot_mapping must be int64")
+    if o != q or odt != qdt:
+        raise ValueError("out must have the query's shape and dtype")
+    if dh > 1 and any(st[-1] != 1 for st in (qst, kst, vst, kcst, vcst, ost)):
+        raise ValueError("channels must be contiguous")
+    if not (_apart(ost, o) and _apart(kcst, kc) and _apart(vcst, vc)):
+        raise ValueError("out and the caches must not have elements that share memory")
+    return ((_A.dtype_code(qdt), N, H, KVH, dh), _lib.i64c(qst[:2]), _lib.i64c(kst[:2]), _lib.i64c(vst[:2]),
+            int(pdt == torch.int64), _lib.i64c(ost[:2]), _A.dtype_code(kcdt), _lib.i64c(kcst[:3]), _lib.i64c(vcst[:3]))

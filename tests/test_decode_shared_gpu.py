@@ -56,6 +56,9 @@ CASES = [  # H, KVH, dh, shared, own lengths
     (4, 1, 128, 4096, [100, 0]),                               # a whole fold segment
     (8, 1, 128, 4300, [0, 4000, 60]),                          # across segments, shared and own
     (4, 2, 64, 8400, [10, 100, 300]),
+    (64, 64, 64, 4300, [0, 5]),                                # enough kv heads that whole segments are folded
+    (128, 64, 128, 4100, [0, 200, 60]),
+    (384, 48, 128, 8500, [30, 1]),                             # two folded segments, then partials
 ]
 
 
@@ -98,6 +101,29 @@ def test_fixture_rows(cut):
             ref = O.decode_rows(q[b], k[:, :cut + x], v[:, :cut + x])
             assert same_bits(got[b], torch.from_numpy(ref).to(DEV)), (c["tag"], b)
         assert H == got.shape[1]
+
+
+@pytest.mark.gpu
+def test_folded_segments_of_fixture_rows():
+    """The same jumps and ladders, tiled past a fold segment over enough kv heads that the segment is folded whole."""
+    for c in jump_cases()[::3] + ftz_cases()[::2]:
+        reps = -(-4200 // c["k"].shape[1])
+        k, v = (np.tile(x, (48, reps, 1))[:, :4200] for x in (c["k"], c["v"]))
+        q = np.tile(c["q"][:1, -1], (48, 1))
+        q = np.stack([q, q * np.float32(0.25)])
+        kv = shared_lattice(k[:, :4100], v[:, :4100], [k[:, 4100:], k[:, 4100:4101]], [v[:, 4100:], v[:, 4100:4101]], False)
+        qt = torch.from_numpy(q).to(DEV)
+        assert same_bits(D.decode_shared(qt, kv, 4100), D.decode(qt, kv)), c["tag"]
+
+
+@pytest.mark.gpu
+def test_queries_that_are_not_finite():
+    q, pk, pv, ks, vs = draw(2, 8, 2, 128, 300, [9, 1], 8)
+    kv = shared_lattice(pk, pv, ks, vs, False)
+    q[0, 1, 3], q[0, 2, 5], q[1, 0], q[1, 7, 64] = np.inf, np.nan, 0.0, -np.inf
+    for dt in (torch.float32, torch.bfloat16, torch.float16):
+        qt = torch.from_numpy(q).to(DEV).to(dt)
+        assert same_bits(D.decode_shared(qt, kv, 300), D.decode(qt, kv))
 
 
 @pytest.mark.gpu

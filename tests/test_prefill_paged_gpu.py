@@ -123,6 +123,35 @@ def test_equals_the_prefill_of_each_sequence_alone():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_queries_that_are_not_finite(dtype):
+    qs, ks, vs = draw([150], [0], 4, 2, 64, 6)
+    qs[0][3, 1, 2], qs[0][4, 0, 0], qs[0][5], qs[0][6, 3, 63] = np.inf, np.nan, 0.0, -np.inf
+    q = torch.from_numpy(qs[0]).to(DEV).to(dtype)
+    t = lambda x: torch.from_numpy(x[None]).to(DEV).to(dtype)                 # noqa: E731
+    alone = A.prefill(q.transpose(0, 1)[None], t(ks[0]), t(vs[0]))[0]
+    assert same_bits(D.prefill_paged(q, lattice(ks, vs, False), cu_of(qs)), alone)
+
+
+@pytest.mark.gpu
+def test_many_short_sequences():
+    """More sequences than the plan's threads, most of them idle or of a single row."""
+    r = np.random.default_rng(3)
+    lens = [int(x) for x in r.choice([1, 2, 17, 128, 130, 257], size=700)]
+    qs, ks, vs = draw(lens, [0] * 700, 2, 1, 64, 12)
+    act = torch.from_numpy(r.random(700) < 0.6).to(DEV)
+    kv, cu = lattice(ks, vs, False), cu_of(qs)
+    q = torch.from_numpy(np.concatenate(qs)).to(DEV)
+    out = D.prefill_paged(q, kv, cu, active=act, out=torch.full_like(q, 4.0))
+    for b in range(0, 700, 23):
+        rows = out[cu[b]:cu[b + 1]]
+        if act[b]:
+            assert same_bits(rows, torch.from_numpy(oracle_rows(qs[b], ks[b], vs[b], 0, 0, False).copy()).to(DEV)), b
+        else:
+            assert (rows == 4.0).all()
+
+
+@pytest.mark.gpu
 def test_strides_idle_sequences_and_untouched_rows():
     lens, T0 = [200, 140, 90, 300], [128, 0, 0, 256]
     qs, ks, vs = draw(lens, T0, 4, 2, 64, 9)
