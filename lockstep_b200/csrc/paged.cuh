@@ -3,6 +3,8 @@
 // and the shared-prefix kernel, are prefill_kernel's paged forms, prefill.cuh; a shared batch's own
 // blocks and refold are the decode kernels' SHARED forms.)
 #pragma once
+#include <type_traits>
+
 #include "decode_tc.cuh"
 #include "prep.cuh"
 
@@ -151,15 +153,27 @@ __global__ void __launch_bounds__(kStepPlanThreads) step_plan_kernel(const Plan 
   pdl_launch_dependents();
   step_plan(plan);
 }
+// max |x| over a 16-byte vector as a bit pattern, NaN included (a pattern above infinity's)
+template <typename InT> __device__ __forceinline__ uint32_t absbits(const uint4& v) {
+  if constexpr (sizeof(InT) == 2) {
+    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+    return max(m & 0xFFFFu, m >> 16);
+  } else {
+    return max(max(v.x & 0x7FFFFFFFu, v.y & 0x7FFFFFFFu), max(v.z & 0x7FFFFFFFu, v.w & 0x7FFFFFFFu));
+  }
+}
 // P1 over tokens [N, H, dh] (strides 0, token, head; contiguous channels, 16-byte rows): row n H + h of q8 and eq.
-// quant_rows_vec's rule with fewer instructions, which bound it here (16,700 tokens of 32 heads: 53 us with its 64-bit
-// row divisions and a conversion an element): the maximum on the bit patterns, and clamp(rint(x 2^e), +-127) as one
-// fused multiply-add onto 1.5 2^23, whose low byte is the rounded integer, clamped as a float (NaN gives -127
-// there and here).
+// quant_rows_vec's rule in fewer instructions, which bound it on these rows (16,700 tokens of 32 bf16 heads: 67 us with
+// its 64-bit row divisions and a conversion an element, 36 us so, 5.7 TB/s): the maximum on the bit patterns, and rint(x 2^e) as
+// one fused multiply-add onto 1.5 2^23, whose low byte is the rounded integer.  |x| 2^e <= 127 by the choice of e,
+// except in a row whose exponent was clamped (e = -32) or that holds a NaN: such a row takes the clamped form, its
+// maximum without the NaN, and NaN gives -127, as there.
 template <typename InT, int DH>
 __device__ __forceinline__ void quant_tokens(int cta, const InT* __restrict__ x, Strides4 xs, int rows, int H,
                                              int8_t* __restrict__ q8, int32_t* __restrict__ eq) {
   constexpr int N = 16 / (int)sizeof(InT), G = DH / N, RPW = 32 / G, RPC = 8 * RPW;
+  constexpr uint32_t kInf = std::is_same<InT, float>::value ? 0x7F800000u : std::is_same<InT, __half>::value ? 0x7C00u : 0x7F80u;
+  constexpr float kMagic = 12582912.0f;                  // 1.5 2^23
   const int sub = threadIdx.x % G;
   const int row0 = cta * RPC * kRowsPerLane + threadIdx.x / G;
   const bool flat = xs.s1 == H * xs.s2;                  // consecutive rows a head stride apart
@@ -174,20 +188,39 @@ __device__ __forceinline__ void quant_tokens(int cta, const InT* __restrict__ x,
 #pragma unroll
   for (int k = 0; k < kRowsPerLane; ++k) {
     const int row = row0 + k * RPC;
-    float m = absmax_value<InT>(absmax_acc<InT>(0u, u[k]));
+    uint32_t bits = absbits<InT>(u[k]);
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const int e = pow2_exponent(m, 40);
+    for (int o = G / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    float m;
+    if constexpr (std::is_same<InT, float>::value) m = __uint_as_float(bits);
+    else if constexpr (std::is_same<InT, __half>::value) m = __half2float(__ushort_as_half((unsigned short)bits));
+    else m = __uint_as_float(bits << 16);
+    int e = pow2_exponent(m, 40);
+    const bool clamp = bits > kInf || e == -32;
+    if (__any_sync(0xffffffffu, clamp)) {                // rare: the maximum without NaN
+      m = absmax_value<InT>(absmax_acc<InT>(0u, u[k]));
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      e = pow2_exponent(m, 40);
+    }
     const float sc = pow2f(e);
     const InT* xe = reinterpret_cast<const InT*>(&u[k]);
-    uint32_t q[N];
+    float y[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      q[i] = __float_as_uint(fminf(fmaxf(__fmaf_rn(to_f32(xe[i]), sc, 12582912.0f), 12582912.0f - 127.0f), 12582912.0f + 127.0f));
+    for (int i = 0; i < N; ++i) y[i] = __fmaf_rn(to_f32(xe[i]), sc, kMagic);
+    if (clamp) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = fminf(fmaxf(y[i], kMagic - 127.0f), kMagic + 127.0f);
+    }
+    uint32_t q[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      q[i] = pack4_s8(__float_as_int(y[4 * i]), __float_as_int(y[4 * i + 1]), __float_as_int(y[4 * i + 2]),
+                      __float_as_int(y[4 * i + 3]));
     if (row < rows) {
       int8_t* dst = q8 + (long long)row * DH + sub * N;
-      if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(pack4_s8(q[0], q[1], q[2], q[3]), pack4_s8(q[4], q[5], q[6], q[7]));
-      else *reinterpret_cast<uint32_t*>(dst) = pack4_s8(q[0], q[1], q[2], q[3]);
+      if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
+      else *reinterpret_cast<uint32_t*>(dst) = q[0];
       if (sub == 0) eq[row] = e;
     }
   }

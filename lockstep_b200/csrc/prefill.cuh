@@ -460,6 +460,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // ================================================================ MMA issuer
     if (lane == 0) {
       constexpr uint32_t kSwz = (DH == 128) ? 2u : 4u;          // 128B / 64B swizzle
+      // The paged forms nap between polls (prefix chunks 532 -> 513 us, packed prompts 1,389 -> 1,380; the dense kernel
+      // loses 1 % by it).
+      constexpr uint32_t kMmaNapNs = PAGED ? 32 : 0;
       constexpr uint32_t kRowGroup = 8 * DH;                    // bytes per 8 rows of a tile
       constexpr uint32_t idesc_qk = idesc_i8(1, 1, 0, 128, 128);
       constexpr uint32_t idesc_pv = idesc_i8(0, 1, PAGED ? 0 : 1, 128, DH);
@@ -472,10 +475,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       auto issue_qk = [&](int jg, uint32_t sq) -> bool {
         const int s = jg & 1;
         const uint32_t ph = (jg >> 1) & 1;
-        if (!mbar_wait(&bars[kBarKFull + s], ph, abort_flag, p.err, 0, p.wait_ns)) return false;
+        if (!mbar_wait(&bars[kBarKFull + s], ph, abort_flag, p.err, kMmaNapNs, p.wait_ns)) return false;
         // S is single-buffered: QK(jg) waits until the chain has copied S(jg - 1) into registers
         // (the jg-th phase of S_empty, jg >= 1)
-        if (jg > 0 && !mbar_wait(&bars[kBarSEmpty], (jg - 1) & 1, abort_flag, p.err, 0, p.wait_ns)) return false;
+        if (jg > 0 && !mbar_wait(&bars[kBarSEmpty], (jg - 1) & 1, abort_flag, p.err, kMmaNapNs, p.wait_ns)) return false;
         tc_fence_after();
         const uint32_t sk = smem_u32(smem + L::kK + s * L::kTile);
 #pragma unroll
@@ -492,7 +495,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         if (!next_item(rd, it)) continue;
         const int nb = PAGED ? it.nb : (GEN && !p.causal) ? p.nblk : it.kt + 1;
         const int qb = tt & 1;
-        if (!mbar_wait(&bars[kBarQFull + qb], (tt >> 1) & 1, abort_flag, p.err, 0, p.wait_ns)) { ok = false; break; }
+        if (!mbar_wait(&bars[kBarQFull + qb], (tt >> 1) & 1, abort_flag, p.err, kMmaNapNs, p.wait_ns)) { ok = false; break; }
         const uint32_t sq = smem_u32(smem + L::kQ + qb * L::kTile);
         ok = issue_qk(jj, sq);
         if (ok && nb == 1) umma_commit(&bars[kBarQEmpty + qb]);   // the item's last QK is issued
@@ -506,10 +509,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           const uint32_t ph = (jg >> 1) & 1;
           const int sa = MULTI ? 0 : s;                             // A buffer and its use parity
           const uint32_t pha = MULTI ? (uint32_t)(jg & 1) : ph;
-          if (!mbar_wait(&bars[kBarPFull + s], ph, abort_flag, p.err, 0, p.wait_ns)) { ok = false; break; }
-          if (!mbar_wait(&bars[kBarVFull + s], ph, abort_flag, p.err, 0, p.wait_ns)) { ok = false; break; }
+          if (!mbar_wait(&bars[kBarPFull + s], ph, abort_flag, p.err, kMmaNapNs, p.wait_ns)) { ok = false; break; }
+          if (!mbar_wait(&bars[kBarVFull + s], ph, abort_flag, p.err, kMmaNapNs, p.wait_ns)) { ok = false; break; }
           // the fold of the block that last used this A buffer is done (jg - 2; jg - 1 in MULTI)
-          if (!mbar_wait(&bars[kBarAEmpty + sa], pha ^ 1, abort_flag, p.err, 0, p.wait_ns)) { ok = false; break; }
+          if (!mbar_wait(&bars[kBarAEmpty + sa], pha ^ 1, abort_flag, p.err, kMmaNapNs, p.wait_ns)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sp = smem_u32(smem + L::kP + s * 16384);
           const uint32_t sv = smem_u32(smem + L::kV + s * L::kTile);
@@ -563,8 +566,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int g = PAGED ? it.g : h / p.group;
       const int nb = PAGED ? it.nb : (GEN && !p.causal) ? p.nblk : kt + 1;   // causal: key blocks 0 .. kt
       const int qb = tt & 1;
-      const int T = PAGED ? it.T : p.T;
-      const bool sink0 = SINK && T > 1 && (!PAGED || it.j0 == 0);   // block 0 of this item holds key 0's own term
+      const bool sink0 = SINK && (PAGED ? it.T : p.T) > 1 && (!PAGED || it.j0 == 0);   // block 0 of this item holds key 0's own term
       // key 0's value row (sink): the item's staged copy, or its channels in the first value page
       const int8_t* v0 = v0row + qb * 128;
       int eqr, srow = 0;                                 // srow (kSrcShared): this row's (sequence, head) pair, or -1
@@ -745,6 +747,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         for (int i = 0; i < 4; ++i) prow_of[i] = __shfl_sync(0xffffffffu, mine, (8 * i + (lane >> 2)) & 15);
       }
       auto store_partials = [&](int jf, int nbb, int lbt, int eh0v) -> bool {
+        if constexpr (SRC != kSrcShared) return true;
         const int jgf = jj0 + jf;
         const int sa = jgf & 1;
         if (!warp_poll(&bars[kBarAFull + sa], (uint32_t)((jgf >> 1) & 1), abort_flag, p.err, p.wait_ns)) return false;
@@ -776,12 +779,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         if (mine >= 0 && kh == 0)
           __stcg(p.pg.partM + mine + (long long)jf * p.group, make_int4(nbb, lbt, sink0 && jf == 0 ? eh0v : 0, 0));
         return true;
-      };
-      auto finish_block = [&](int jf, int nbb, int lbt, int evj, int eh0v, bool live) -> bool {
-        if constexpr (SRC == kSrcShared) {
-          if (!it.fold) return store_partials(jf, nbb, lbt, eh0v);
-        }
-        return fold_block(jf, nbb, lbt, evj, eh0v, live);
       };
       int nb_prev = 0, ev_prev = 0, lbt_prev = 0, eh0_row = 0;
       bool live_prev = true;
@@ -904,13 +901,19 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const uint32_t lb = lbq[0] + lbq[1];
         const int lbt = (int)lb + __shfl_xor_sync(0xffffffffu, (int)lb, 16);   // the row's l_b
         if (SINK && j == 0) eh0_row = __shfl_sync(0xffffffffu, (int)eh0, lane & 15);
-        if (j > 0 && !finish_block(j - 1, nb_prev, lbt_prev, ev_prev, eh0_row, live_prev)) { ok = false; break; }
+        if (SRC == kSrcShared && !it.fold) {               // block j - 1's partials, or its fold
+          if (j > 0 && !store_partials(j - 1, nb_prev, lbt_prev, eh0_row)) { ok = false; break; }
+        } else if (j > 0 && !fold_block(j - 1, nb_prev, lbt_prev, ev_prev, eh0_row, live_prev)) { ok = false; break; }
         nb_prev = nbv;
         lbt_prev = lbt;
         ev_prev = evj;
         live_prev = live;
       }
-      if (ok) ok = finish_block(nb - 1, nb_prev, lbt_prev, ev_prev, eh0_row, live_prev);
+      if (SRC == kSrcShared && !it.fold) {
+        if (ok) ok = store_partials(nb - 1, nb_prev, lbt_prev, eh0_row);
+      } else if (ok) {
+        ok = fold_block(nb - 1, nb_prev, lbt_prev, ev_prev, eh0_row, live_prev);
+      }
 
       // ---- epilogue: out = O_row / l_row (one RN division per element; l_row == 0 -> 0).
       // `ok` is warp-uniform (every wait is decided for the whole warp), so the warp-collective
@@ -937,7 +940,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       } else if (ok) {
         if (!mseg) lrow = rescale(lseg, 0);             // a single segment: O_row = 0 + rescale(O_seg, 0)
         const int i = kt * 128 + r;                      // the row's position in the sequence
-        const bool live = (i < T);
+        const bool live = (i < (PAGED ? it.T : p.T));
         const bool nz = (lrow != 0.0f);
         const float rl = nz ? __frcp_rn(lrow) : 0.0f;
         const bool row_fast = div_window(lrow);

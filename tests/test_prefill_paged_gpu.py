@@ -127,6 +127,10 @@ def test_equals_the_prefill_of_each_sequence_alone():
 def test_queries_that_are_not_finite(dtype):
     qs, ks, vs = draw([150], [0], 4, 2, 64, 6)
     qs[0][3, 1, 2], qs[0][4, 0, 0], qs[0][5], qs[0][6, 3, 63] = np.inf, np.nan, 0.0, -np.inf
+    qs[0][7] *= np.float32(2.0 ** 60)                          # past the exponent's clamp (infinite in float16)
+    qs[0][8] *= np.float32(2.0 ** -130)                        # subnormal (zero in float16)
+    qs[0][9, 2, 5:9] = np.nan
+    qs[0][9, 2, 9] = -300.0
     q = torch.from_numpy(qs[0]).to(DEV).to(dtype)
     t = lambda x: torch.from_numpy(x[None]).to(DEV).to(dtype)                 # noqa: E731
     alone = A.prefill(q.transpose(0, 1)[None], t(ks[0]), t(vs[0]))[0]
