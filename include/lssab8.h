@@ -288,7 +288,7 @@ int lssab8_rotate(const void* x, int dtype, int B, int H, int T, int dh, const i
  * v copied into the engine's paged float cache, k_cache / v_cache [num_pages, 16, KVH, dh] (strides kcs / vcs of
  * the first three dimensions, channels contiguous) in cache_dtype, at slot page * 16 + row.  Slot -1 (the padded
  * end of a step) stores nothing; any other slot outside the cache sets LSSAB8_DEV_BAD_PAGE and stores nothing.
- * Two tokens with one slot: either is stored.  qs / ks / vs / os: token and head strides, channels contiguous. */
+ * Two tokens with one slot leave a mix of both.  qs / ks / vs / os: token and head strides, channels contiguous. */
 int lssab8_rotate_append(const void* q, const void* k, const void* v, int dtype, int N, int H, int KVH, int dh,
                          const int64_t* qs, const int64_t* ks, const int64_t* vs, const void* positions, int pos64,
                          int64_t pos_stride, const uint64_t* freq, float factor, int rot, int layout, void* q_out,

@@ -5,6 +5,7 @@ liblssab8_b200.so.  Tensors must be CUDA tensors of one floating dtype (float32 
 bfloat16); anything else raises -- there is no CPU path.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -22,7 +23,9 @@ def dtype_code(dt):
 
 
 def _stream_handle(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)      # current_stream(device).cuda_stream, 2.6 us cheaper
+    if isinstance(device, torch.device) and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)  # current_stream's handle, 2.6 us cheaper
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 class _Here:
@@ -41,6 +44,21 @@ _HERE = _Here()
 def _on(device):
     """torch.cuda.device(device), without its cost when the device is current already."""
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _apart(strides, shape):
+    end = 0
+    for st, n in sorted((st, n) for st, n in zip(strides, shape) if n > 1):
+        if st <= end:
+            return False
+        end += st * (n - 1)
+    return True
+
+
+def _written_once(t):
+    """No two elements of t share memory (as far as strides tell)."""
+    return _apart(t.stride(), t.shape)
 
 
 def _require_cuda(*ts):

@@ -358,10 +358,9 @@ int lssab8_step_tables(const int32_t* before, const int32_t* fresh, int n, int32
   const TablesArgs a{before, fresh, n, max_pages, nfree, cap, block_table, table_stride, free_pages, query_start_loc,
                      seq_lens, seq_index, pages_used, reinterpret_cast<long long*>(slot_mapping),
                      reinterpret_cast<long long*>(positions), ds->err};
+  static SmemAttr attr;                                       // (the most any call needs: calls may run side by side)
+  if (!attr.set(step_tables_kernel, (3 * kTblMaxSeqs + 2) * 4)) return kErrCuda;
   const int smem = (3 * n + 2) * 4;
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return kErrCuda;
   const int grid = std::max(1, std::min((cap + kTblThreads - 1) / kTblThreads, ds->num_sms));
   step_tables_kernel<<<grid, kTblThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
   return launch_rc();

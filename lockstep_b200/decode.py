@@ -230,8 +230,8 @@ def _check_lattice(q, kv, B, H, dh):
 
 
 def _check_out(out, shape, dev):
-    if out.shape != shape or out.device != dev:
-        raise ValueError("out must be %s on the query's device" % (tuple(shape),))
+    if out.shape != shape or out.device != dev or not _A._written_once(out):
+        raise ValueError("out must be %s on the query's device, with no shared elements" % (tuple(shape),))
 
 
 def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtype=None, check=True):

@@ -82,21 +82,6 @@ def _check_positions(positions):
         raise TypeError("positions must be int32 or int64, got %s" % positions.dtype)
 
 
-@functools.lru_cache(maxsize=4096)
-def _apart(strides, shape):
-    end = 0
-    for st, n in sorted((st, n) for st, n in zip(strides, shape) if n > 1):
-        if st <= end:
-            return False
-        end += st * (n - 1)
-    return True
-
-
-def _written_once(t):
-    """No two elements of t share memory (as far as strides tell)."""
-    return _apart(t.stride(), t.shape)
-
-
 def _launch(x, positions, plan, inverse, out):
     dev = _A._require_cuda(x, positions, plan.freq, out)
     if x.numel() == 0:
@@ -130,7 +115,9 @@ def rotate(x, positions, plan, inverse=False, out=None):
     """x [B, H, T, dh] with positions [T] or [B, T], or x [N, H, dh] with positions [N] -> rotated x, same type
     and shape (any strides; float32, float16, bfloat16).  inverse=True: the transposed map (it undoes
     the rotation when the plan's factor is 1); differentiable in x, the gradient being the other direction.
-    out: written instead (out=x rotates in place); not with a gradient."""
+    out: written instead (out=x rotates in place); not with a gradient.  In a captured graph: torch refuses to capture a
+    backward pass while an eager graph of the same leaf is alive; rotate(g, positions, plan, inverse=True) is the same
+    gradient and needs no graph of the leaf."""
     if x.dim() not in (3, 4) or x.shape[-1] != plan.head_dim:
         raise ValueError("x must be [B, H, T, %d] or [N, H, %d], got %s" % (plan.head_dim, plan.head_dim, tuple(x.shape)))
     _check_positions(positions)
@@ -146,7 +133,7 @@ def rotate(x, positions, plan, inverse=False, out=None):
         out = torch.empty_like(x, memory_format=torch.preserve_format)
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("out must have x's shape and dtype")
-    if not _written_once(out):
+    if not _A._written_once(out):
         raise ValueError("out has elements that share memory")
     return _launch(x, positions, plan, inverse, out)
 
@@ -155,7 +142,8 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
     """A serving step's new tokens: query [N, H, dh] rotated (returned, or written to out, which may be
     query), key [N, KVH, dh] rotated and value [N, KVH, dh] stored in k_cache / v_cache [num_pages, 16, KVH, dh]
     (any page, row and head strides; the cache's own dtype, one rounding) at slot_mapping [N] int64, page * 16 +
-    row.  Slot -1 stores nothing.  Inference only: no gradient flows through it."""
+    row.  Slot -1 stores nothing; the other slots must differ (two tokens in one slot leave a mix of both).  Inference
+    only: no gradient flows through it."""
     dev = _A._require_cuda(query, key, value, positions, slot_mapping, k_cache, v_cache, plan.freq)
     if (query.requires_grad or key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
         raise ValueError("rotate_append has no gradient (use rotate)")
@@ -207,7 +195,7 @@ def _append_args(q, qst, qdt, k, kst, kdt, v, vst, vdt, kc, kcst, kcdt, vc, vcst
         raise ValueError("out must have the query's shape and dtype")
     if dh > 1 and any(st[-1] != 1 for st in (qst, kst, vst, kcst, vcst, ost)):
         raise ValueError("channels must be contiguous")
-    if not (_apart(ost, o) and _apart(kcst, kc) and _apart(vcst, vc)):
+    if not (_A._apart(ost, o) and _A._apart(kcst, kc) and _A._apart(vcst, vc)):
         raise ValueError("out and the caches must not have elements that share memory")
     return ((_A.dtype_code(qdt), N, H, KVH, dh), _lib.i64c(qst[:2]), _lib.i64c(kst[:2]), _lib.i64c(vst[:2]),
             int(pdt == torch.int64), _lib.i64c(ost[:2]), _A.dtype_code(kcdt), _lib.i64c(kcst[:3]), _lib.i64c(vcst[:3]))

@@ -8,6 +8,7 @@ import torch
 import oracle as O
 from fixtures import ftz_cases, jump_cases
 from lockstep_b200 import _lib
+from lockstep_b200 import attention as A
 from lockstep_b200 import decode as D
 from lockstep_b200 import workloads as W
 
@@ -179,6 +180,10 @@ def test_strided_queries_and_outputs():
     assert same_bits(out, want)
     with pytest.raises(ValueError):
         D.decode_shared(qt, kv, 260, out=torch.zeros(3, 8, 64, device=DEV))
+    with pytest.raises(ValueError):
+        D.decode_shared(qt, kv, 260, out=torch.zeros(3, 1, 128, device=DEV).expand(3, 8, 128))
+    for dev in (None, "cuda", torch.device("cuda"), qt.device):        # every way to name the device
+        A.check_device_errors(dev)
     with pytest.raises(ValueError):
         D.decode_shared(qt, kv, 128 * (kv.max_blocks + 1))
     with pytest.raises(ValueError):

@@ -203,4 +203,18 @@ def test_streams_and_graph():
     pos += 1000
     graph.replay()
     assert torch.equal(y, R.rotate(x, pos, plan)) and torch.equal(z, R.rotate(y, pos, plan, inverse=True))
+    # a captured backward pass, and the gradient captured directly while an eager graph of the leaf lives
+    leaf, g = x.float().requires_grad_(True), torch.randn(8, 4, 128, device="cuda")
+    want = R.rotate(g, pos, plan, inverse=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(R.rotate(leaf, pos, plan), leaf, g)
+    graph.replay()
+    assert torch.equal(got, want)
+    alive = R.rotate(leaf, pos, plan)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = R.rotate(g, pos, plan, inverse=True)
+    graph.replay()
+    assert torch.equal(got, want) and torch.equal(torch.autograd.grad(alive, leaf, g)[0], want)
     assert D.PAGE == R.PAGE and math.isfinite(float(z.float().sum()))
