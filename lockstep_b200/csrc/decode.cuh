@@ -139,8 +139,9 @@ __device__ __forceinline__ void decode_merge_head(const DecodeArgs& p, int b, in
 }
 
 // SHARED: only the blocks after the shared ones, whose partials alone are stored (the refold is
-// decode_merge_kernel, decode_tc.cuh).  It runs beside the shared-prefix kernel before it, and completes after it
-// (every CTA's wait), so that the refold's wait covers both.
+// decode_merge_kernel, decode_tc.cuh).  It runs beside the shared-prefix kernel before it, which lets it start once the
+// queries are quantised and whose output it does not read; every CTA waits for that kernel before it ends, so the
+// refold, ordered after this grid alone in a captured graph, comes after both.  (Small batches: 18.1 -> 14.9 us.)
 template <int DH, bool SINK, typename OutT, bool SHARED = false>
 __global__ void __launch_bounds__(128)
 decode_kernel(const DecodeArgs p) {
