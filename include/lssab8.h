@@ -318,7 +318,7 @@ size_t lssab8_prefill_paged_workspace_size(int N, int H, int KVH, int dh, int B)
  * contract's row over these keys: without a prefix, bit-identical to lssab8_prefill of the sequence alone.
  * active [B] (NULL: all): sequences with 0 have no rows here.  Rows of q that belong to no such sequence, and
  * sequences that break a rule (LSSAB8_DEV_PLAN / LSSAB8_DEV_BAD_PAGE), leave out as it was.  out [N, H, dh].
- * Lattice arguments as in lssab8_decode; any group; dh in {64, 128}. */
+ * Lattice arguments as in lssab8_decode (k8p and v8p 16-byte aligned); any group; dh in {64, 128}. */
 int lssab8_prefill_paged(const void* q, int dtype, const int64_t* qs, int N, int H, int KVH, int dh, const int32_t* cu_q,
                          const int32_t* seq_lens, const int32_t* prefix_lens, const uint8_t* active, int B,
                          const int32_t* block_table, int max_pages, int num_pages, const int8_t* k8p,

@@ -379,7 +379,8 @@ int lssab8_prefill_paged(const void* q, int dtype, const int64_t* qs, int N, int
                          void* stream) {
   if (!q || !cu_q || !seq_lens || !block_table || !k8p || !v8p || !ek || !ev || (sink && !ev0) || !out || !workspace ||
       !strides_ok(qs, 3) || !strides_ok(os, 3) || B <= 0 || !shape_ok(1, H, KVH, N, dh) || max_blocks <= 0 ||
-      max_pages <= 0 || num_pages <= 0 || (long long)num_pages * KVH * 16 > 0x7FFFFFFFll ||
+      max_pages <= 0 || num_pages <= 0 || (long long)num_pages * KVH * 16 > 0x7FFFFFFFll || !aligned16(k8p) ||
+      !aligned16(v8p) ||
       (long long)H * N > 0x7FFFFFFFll || ((long long)N / 128 + B) * H > 0x7FFFFFFFll)
     return kErrArg;
   if (dh != 64 && dh != 128) return kErrUnsupported;
@@ -429,7 +430,7 @@ int lssab8_decode_shared(const void* q, int dtype, const int64_t* qs, int B, int
                          void* workspace, size_t workspace_bytes, void* stream) {
   if (!q || !seq_lens || !block_table || !k8p || !v8p || !ek || !ev || (sink && !ev0) || !out || !workspace ||
       !strides_ok(qs, 3) || !strides_ok(os, 3) || max_pages <= 0 || num_pages <= 0 ||
-      (long long)num_pages * KVH * 16 > 0x7FFFFFFFll)
+      (long long)num_pages * KVH * 16 > 0x7FFFFFFFll || !aligned16(k8p) || !aligned16(v8p))
     return kErrArg;
   SharedShape sh;
   SharedWs w;

@@ -11,6 +11,7 @@ Lattice layout (16-key pages; KB = 128 keys = 8 pages per contract block):
     ek, ev [B, KVH, max_blocks]    int32 per logical 128-key block; ev0 [B, KVH] (sink)
     block_table [B, max_pages]     int32 physical page of each logical page (-1 = none)
 """
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -212,21 +213,29 @@ def decode(q, kv, split_blocks=4, out=None, out_dtype=None, check=True):
     return out
 
 
-def _check_lattice(q, kv, B, H, dh):
-    """Checks q [.., H, dh] against the lattice; returns (device, KVH)."""
-    k8p, lens, table, ek, ev, ev0 = kv.k8p, kv.seq_lens, kv.block_table, kv.ek, kv.ev, kv.ev0
-    dev = _A._require_cuda(q, k8p, kv.v8p, lens, table, ek, ev, ev0)
-    pages, KVH, _, lat_dh = k8p.shape
-    if (dh != lat_dh or H % KVH or lens.shape != (B,) or table.dim() != 2 or table.shape[0] != B or
-            ek.shape != (B, KVH, kv.max_blocks) or ev.shape != ek.shape or ev0.shape != (B, KVH) or pages < kv.num_pages):
+@functools.lru_cache(maxsize=1024)
+def _lattice_fits(H, dh, k8p, v8p, lens, table, ek, ev, ev0, max_blocks, num_pages):
+    """The shapes of a lattice and a query that belong together; kept, since a model's steps repeat them."""
+    pages, KVH, page, lat_dh = k8p
+    B = lens[0] if len(lens) == 1 else -1
+    return (dh == lat_dh and page == PAGE and H % KVH == 0 and v8p == (pages, KVH, dh, PAGE) and len(table) == 2 and
+            table[0] == B and ek == (B, KVH, max_blocks) and ev == ek and ev0 == (B, KVH) and pages >= num_pages)
+
+
+def _check_lattice(q, kv, H, dh):
+    """Checks q [.., H, dh] against the lattice; returns (device, kv heads)."""
+    k8p, v8p, lens, table, ek, ev, ev0 = kv.k8p, kv.v8p, kv.seq_lens, kv.block_table, kv.ek, kv.ev, kv.ev0
+    dev = _A._require_cuda(q, k8p, v8p, lens, table, ek, ev, ev0)
+    if not _lattice_fits(H, dh, k8p.shape, v8p.shape, lens.shape, table.shape, ek.shape, ev.shape, ev0.shape,
+                         kv.max_blocks, kv.num_pages):
         raise ValueError("query does not match the lattice")
     if not (lens.is_contiguous() and table.is_contiguous() and ek.is_contiguous() and ev.is_contiguous() and
-            ev0.is_contiguous() and k8p.is_contiguous() and kv.v8p.is_contiguous()):
+            ev0.is_contiguous() and k8p.is_contiguous() and v8p.is_contiguous()):
         raise ValueError("the lattice's pages, lengths, table and exponents must be contiguous")
     i32 = torch.int32
     if lens.dtype != i32 or table.dtype != i32 or ek.dtype != i32 or ev.dtype != i32 or ev0.dtype != i32:
         raise TypeError("the lattice's lengths, table and exponents must be int32")
-    return dev, KVH
+    return dev, k8p.shape[1]
 
 
 def _check_out(out, shape, dev):
@@ -249,7 +258,7 @@ def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtyp
         raise ValueError("q must be [N, H, dh]")
     N, H, dh = q.shape
     B = kv.seq_lens.numel()
-    dev, KVH = _check_lattice(q, kv, B, H, dh)
+    dev, KVH = _check_lattice(q, kv, H, dh)
     _A._require_cuda(q, cu_q, *[t for t in (prefix_lens, active) if t is not None])
     if cu_q.shape != (B + 1,) or cu_q.dtype != torch.int32:
         raise ValueError("cu_q must be [%d] int32" % (B + 1))
@@ -303,7 +312,9 @@ def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
         raise ValueError("shared_len must not be negative")
     if shared_len < KB:
         return decode(q, kv, out=out, out_dtype=out_dtype, check=check)
-    dev, KVH = _check_lattice(q, kv, B, H, dh)
+    dev, KVH = _check_lattice(q, kv, H, dh)
+    if kv.seq_lens.shape[0] != B:
+        raise ValueError("query does not match the lattice")
     if shared_len // KB > kv.max_blocks or shared_len // KB * (KB // PAGE) > kv.block_table.shape[1]:
         raise ValueError("the lattice holds at most %d blocks a sequence" % kv.max_blocks)
     if out is None:

@@ -232,11 +232,12 @@ def test_c_entry_refusals():
     L = _lib.load()
     s, f = _lib.i64x([1, 1, 1]), 256
 
-    def call(B=2, H=4, KVH=2, dh=64, shared=128, mp=8, npg=8, mb=1, sink=0, ev0=f, q=f):
-        return L.lssab8_decode_shared(q, 2, s, B, H, KVH, dh, f, shared, f, mp, npg, f, f, f, f, ev0, mb, sink, f, 2, s, f,
+    def call(B=2, H=4, KVH=2, dh=64, shared=128, mp=8, npg=8, mb=1, sink=0, ev0=f, q=f, k8=f, v8=f):
+        return L.lssab8_decode_shared(q, 2, s, B, H, KVH, dh, f, shared, f, mp, npg, k8, v8, f, f, ev0, mb, sink, f, 2, s, f,
                                       1 << 40, None)
     for kw in (dict(B=0), dict(H=3), dict(shared=127), dict(shared=256), dict(mb=0), dict(mp=0), dict(npg=0),
-               dict(npg=1 << 27), dict(q=None), dict(sink=1, ev0=None), dict(B=70000)):
+               dict(npg=1 << 27), dict(q=None), dict(sink=1, ev0=None), dict(B=70000), dict(k8=f + 8),
+               dict(v8=f + 1)):
         assert call(**kw) == 1, kw
     assert call(dh=96) == 2 and call(H=18, KVH=2) == 2
     assert L.lssab8_decode_shared_workspace_size(2, 4, 2, 64, 1, 127) == 0

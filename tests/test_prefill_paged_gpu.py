@@ -259,11 +259,11 @@ def test_c_entry_refusals():
     L = _lib.load()
     s, f = _lib.i64x([1, 1, 1]), 256
 
-    def call(N=10, H=4, KVH=2, dh=64, B=1, mb=1, mp=8, npg=8, sink=0, ev0=f, q=f, ws=1 << 30):
-        return L.lssab8_prefill_paged(q, 2, s, N, H, KVH, dh, f, f, None, None, B, f, mp, npg, f, f, f, f, ev0, mb, sink, f, 2,
-                                      s, f, ws, None)
+    def call(N=10, H=4, KVH=2, dh=64, B=1, mb=1, mp=8, npg=8, sink=0, ev0=f, q=f, ws=1 << 30, k8=f, v8=f):
+        return L.lssab8_prefill_paged(q, 2, s, N, H, KVH, dh, f, f, None, None, B, f, mp, npg, k8, v8, f, f, ev0, mb, sink, f,
+                                      2, s, f, ws, None)
     for kw in (dict(N=0), dict(H=3), dict(B=0), dict(mb=0), dict(mp=0), dict(npg=0), dict(npg=1 << 27), dict(q=None),
-               dict(sink=1, ev0=None)):
+               dict(sink=1, ev0=None), dict(k8=f + 8), dict(v8=f + 1)):
         assert call(**kw) == 1, kw
     assert call(dh=96) == 2 and call(ws=100) == 4
     assert L.lssab8_prefill_paged_workspace_size(0, 4, 2, 64, 1) == 0
