@@ -50,6 +50,9 @@ def build(force=False, verbose=False):
         r = subprocess.run([nvcc(), "-shared", "-o", LIB] + NVCC_FLAGS[:2] + objs, cwd=CSRC, capture_output=True, text=True)
         logs.append(r.stdout + r.stderr)
         jobs.append(r)
+    for o in objs:
+        if os.path.exists(o):
+            os.remove(o)
     if any(j.returncode != 0 for j in jobs):
         sys.stderr.write("".join(logs))
         raise RuntimeError("nvcc failed building liblssab8_b200.so")
