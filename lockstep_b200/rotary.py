@@ -103,12 +103,14 @@ class _Rotate(torch.autograd.Function):
     def forward(ctx, x, positions, plan, inverse):
         ctx.save_for_backward(positions)
         ctx.plan, ctx.inverse = plan, inverse
-        return _launch(x, positions, plan, inverse, torch.empty_like(x, memory_format=torch.preserve_format))
+        return _launch(x, positions, plan, inverse, torch.empty_like(x))
 
     @staticmethod
     def backward(ctx, g):
         positions, = ctx.saved_tensors
-        return rotate(g, positions, ctx.plan, inverse=not ctx.inverse), None, None, None
+        if torch.is_grad_enabled():                              # a gradient of the gradient is wanted
+            return rotate(g, positions, ctx.plan, inverse=not ctx.inverse), None, None, None
+        return _launch(g, positions, ctx.plan, not ctx.inverse, torch.empty_like(g)), None, None, None
 
 
 def rotate(x, positions, plan, inverse=False, out=None):
@@ -118,20 +120,20 @@ def rotate(x, positions, plan, inverse=False, out=None):
     out: written instead (out=x rotates in place); not with a gradient.  In a captured graph: torch refuses to capture a
     backward pass while an eager graph of the same leaf is alive; rotate(g, positions, plan, inverse=True) is the same
     gradient and needs no graph of the leaf."""
-    if x.dim() not in (3, 4) or x.shape[-1] != plan.head_dim:
-        raise ValueError("x must be [B, H, T, %d] or [N, H, %d], got %s" % (plan.head_dim, plan.head_dim, tuple(x.shape)))
+    shape, ps = x.shape, positions.shape
+    if len(shape) not in (3, 4) or shape[-1] != plan.head_dim:
+        raise ValueError("x must be [B, H, T, %d] or [N, H, %d], got %s" % (plan.head_dim, plan.head_dim, tuple(shape)))
     _check_positions(positions)
-    want = [(x.shape[0],)] if x.dim() == 3 else [(x.shape[2],), (x.shape[0], x.shape[2])]
-    if tuple(positions.shape) not in want:
-        raise ValueError("positions must be %s, got %s" % (" or ".join(map(str, want)), tuple(positions.shape)))
+    if ps != (shape[0] if len(shape) == 3 else shape[2],) and (len(shape) == 3 or ps != (shape[0], shape[2])):
+        raise ValueError("positions must be [N], [T] or [B, T] for x %s, got %s" % (tuple(shape), tuple(ps)))
     _A.dtype_code(x.dtype)
     if torch.is_grad_enabled() and x.requires_grad:
         if out is not None:
             raise ValueError("out= has no gradient: rotate a detached tensor, or leave out away")
         return _Rotate.apply(x, positions, plan, bool(inverse))
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.preserve_format)
-    elif out.shape != x.shape or out.dtype != x.dtype:
+        return _launch(x, positions, plan, inverse, torch.empty_like(x))
+    if out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("out must have x's shape and dtype")
     if not _A._written_once(out):
         raise ValueError("out has elements that share memory")
