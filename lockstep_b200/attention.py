@@ -90,17 +90,10 @@ def check_device_errors(device=None):
                            "request lengths or prefixes that do not fit=16)" % bits)
 
 
-_WS = {}
-
-
 def workspace(device, nbytes):
-    """A cached uint8 device buffer of at least nbytes (grown, never shrunk)."""
-    key = (device.type, device.index)
-    buf = _WS.get(key)
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
-        _WS[key] = buf
-    return buf
+    """A uint8 device buffer of at least nbytes for one call, from torch's allocator on the current stream: calls on
+    other streams and captured graphs never write the same one."""
+    return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
 
 
 def quant_rows(x, Tpad=None):

@@ -1,0 +1,57 @@
+"""The host layer of the serving-step operators without a GPU: the library is a stand-in that records its calls, so what
+is tested is everything around the kernels (workspaces, checks, gradients, versions), on CPU tensors."""
+import pytest
+import torch
+
+from lockstep_b200 import _lib
+from lockstep_b200 import attention as A
+from lockstep_b200 import decode as D
+
+
+class Recorder:
+    """Every entry point succeeds and is recorded as (name, arguments); a size query answers 4096."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.calls.append((name, args))
+            return 4096 if name.endswith("workspace_size") else 0
+        return entry
+
+    def names(self):
+        return [n for n, _ in self.calls if not n.endswith("workspace_size")]
+
+
+class Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    rec = Recorder()
+    monkeypatch.setattr(_lib, "load", lambda: rec)
+    monkeypatch.setattr(A, "_require_cuda", lambda *ts: ts[0].device)
+    monkeypatch.setattr(A, "_on", lambda dev: Here())
+    monkeypatch.setattr(A, "_stream_handle", lambda dev: 0)
+    monkeypatch.setattr(A, "check_device_errors", lambda dev=None: None)
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: Here())
+    return rec
+
+
+def lattice(B=2, KVH=2, dh=64, blocks=4, pages=40, sink=False):
+    kv = D.empty_paged_kv(B, KVH, dh, blocks * 128, torch.zeros((B, blocks * 8), dtype=torch.int32), pages, sink=sink)
+    kv.seq_lens.fill_(300)
+    return kv
+
+
+def test_every_call_has_a_workspace_of_its_own():
+    """Two calls in flight (two streams, or two captured graphs) never write one buffer."""
+    a = A.workspace(torch.device("cpu"), 64)
+    b = A.workspace(torch.device("cpu"), 32)
+    assert a.numel() >= 64 and b.numel() >= 32 and a.data_ptr() != b.data_ptr()
