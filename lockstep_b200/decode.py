@@ -310,11 +310,13 @@ def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
     shared_len = int(shared_len)
     if shared_len < 0:
         raise ValueError("shared_len must not be negative")
-    if shared_len < KB:
-        return decode(q, kv, out=out, out_dtype=out_dtype, check=check)
     dev, KVH = _check_lattice(q, kv, H, dh)
     if kv.seq_lens.shape[0] != B:
         raise ValueError("query does not match the lattice")
+    if shared_len < KB:
+        if out is not None:
+            _check_out(out, q.shape, dev)
+        return decode(q, kv, out=out, out_dtype=out_dtype, check=check)
     if shared_len // KB > kv.max_blocks or shared_len // KB * (KB // PAGE) > kv.block_table.shape[1]:
         raise ValueError("the lattice holds at most %d blocks a sequence" % kv.max_blocks)
     if out is None:

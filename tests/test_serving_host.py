@@ -55,3 +55,24 @@ def test_every_call_has_a_workspace_of_its_own():
     a = A.workspace(torch.device("cpu"), 64)
     b = A.workspace(torch.device("cpu"), 32)
     assert a.numel() >= 64 and b.numel() >= 32 and a.data_ptr() != b.data_ptr()
+
+
+@pytest.mark.parametrize("shared", [0, 100, 200])
+def test_decode_shared_checks_its_arguments_at_every_prefix_length(lib, shared):
+    q, kv = torch.zeros(2, 4, 64), lattice()
+    D.decode_shared(q, kv, shared)
+    assert lib.names() == ["lssab8_decode" if shared < 128 else "lssab8_decode_shared"]
+    del lib.calls[:]
+    for out in (torch.zeros(2, 4, 32), torch.zeros(1, 4, 64), torch.zeros(2, 1, 64).expand(2, 4, 64)):
+        with pytest.raises(ValueError):
+            D.decode_shared(q, kv, shared, out=out)
+    wide = lattice()
+    wide.block_table = torch.zeros((2, 64), dtype=torch.int32)[:, :32]           # rows that are not next to each other
+    cut = lattice()
+    cut.ek = torch.zeros((2, 2, 8), dtype=torch.int32)[..., ::2]
+    half = lattice()
+    half.ev = half.ev.to(torch.int16)
+    for bad in (wide, cut, half, lattice(B=3), lattice(dh=128), lattice(KVH=3)):
+        with pytest.raises((ValueError, TypeError)):
+            D.decode_shared(q, bad, shared)
+    assert not lib.names()
