@@ -8,6 +8,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad as _fwd
 
 from . import _lib
 
@@ -59,6 +60,13 @@ def _apart(strides, shape):
 def _written_once(t):
     """No two elements of t share memory (as far as strides tell)."""
     return _apart(t.stride(), t.shape)
+
+
+def _differentiable(*ts):
+    """A derivative would have to flow through one of ts: it requires a gradient, or carries a forward-mode tangent."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        return True
+    return _fwd._current_level >= 0 and any(_fwd.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _require_cuda(*ts):

@@ -102,6 +102,7 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, plan, inverse):
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.plan, ctx.inverse = plan, inverse
         return _launch(x, positions, plan, inverse, torch.empty_like(x))
 
@@ -112,11 +113,17 @@ class _Rotate(torch.autograd.Function):
             return rotate(g, positions, ctx.plan, inverse=not ctx.inverse), None, None, None
         return _launch(g, positions, ctx.plan, not ctx.inverse, torch.empty_like(g)), None, None, None
 
+    @staticmethod
+    def jvp(ctx, t, *_):                                         # the map is linear: the tangent is rotated as x is
+        positions, = ctx.saved_tensors
+        return rotate(t, positions, ctx.plan, inverse=ctx.inverse)
+
 
 def rotate(x, positions, plan, inverse=False, out=None):
     """x [B, H, T, dh] with positions [T] or [B, T], or x [N, H, dh] with positions [N] -> rotated x, same type
     and shape (any strides; float32, float16, bfloat16).  inverse=True: the transposed map (it undoes
-    the rotation when the plan's factor is 1); differentiable in x, the gradient being the other direction.
+    the rotation when the plan's factor is 1); differentiable in x, the gradient being the other direction
+    (forward mode: the tangent is rotated too).
     out: written instead (out=x rotates in place); not with a gradient.  In a captured graph: torch refuses to capture a
     backward pass while an eager graph of the same leaf is alive; rotate(g, positions, plan, inverse=True) is the same
     gradient and needs no graph of the leaf."""
@@ -127,7 +134,7 @@ def rotate(x, positions, plan, inverse=False, out=None):
     if ps != (shape[0] if len(shape) == 3 else shape[2],) and (len(shape) == 3 or ps != (shape[0], shape[2])):
         raise ValueError("positions must be [N], [T] or [B, T] for x %s, got %s" % (tuple(shape), tuple(ps)))
     _A.dtype_code(x.dtype)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _A._differentiable(x):
         if out is not None:
             raise ValueError("out= has no gradient: rotate a detached tensor, or leave out away")
         return _Rotate.apply(x, positions, plan, bool(inverse))
@@ -147,7 +154,7 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
     row.  Slot -1 stores nothing; the other slots must differ (two tokens in one slot leave a mix of both).  Inference
     only: no gradient flows through it."""
     dev = _A._require_cuda(query, key, value, positions, slot_mapping, k_cache, v_cache, plan.freq)
-    if (query.requires_grad or key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
+    if _A._differentiable(query, key, value):
         raise ValueError("rotate_append has no gradient (use rotate)")
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)

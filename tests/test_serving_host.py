@@ -2,10 +2,12 @@
 is tested is everything around the kernels (workspaces, checks, gradients, versions), on CPU tensors."""
 import pytest
 import torch
+from torch.autograd import forward_ad as fwd
 
 from lockstep_b200 import _lib
 from lockstep_b200 import attention as A
 from lockstep_b200 import decode as D
+from lockstep_b200 import rotary as R
 
 
 class Recorder:
@@ -75,4 +77,57 @@ def test_decode_shared_checks_its_arguments_at_every_prefix_length(lib, shared):
     for bad in (wide, cut, half, lattice(B=3), lattice(dh=128), lattice(KVH=3)):
         with pytest.raises((ValueError, TypeError)):
             D.decode_shared(q, bad, shared)
+    assert not lib.names()
+
+
+def plain_rotation(x, positions, plan, inverse, out):
+    """rotary._launch in elementary operations, half layout."""
+    n = plan.rotary_dim // 2
+    theta = torch.tensor(R.frequencies(plan.rotary_dim)[0], dtype=torch.float64)
+    a = positions.double()[:, None] * theta * (-1.0 if inverse else 1.0)
+    with torch.no_grad():
+        x = x.detach()
+        c, s, x1, x2 = a.cos(), a.sin(), x[..., :n].double(), x[..., n:2 * n].double()
+        out[..., :n], out[..., n:2 * n], out[..., 2 * n:] = x1 * c - x2 * s, x2 * c + x1 * s, x[..., 2 * n:]
+    return out
+
+
+@pytest.fixture
+def rotation(monkeypatch):
+    monkeypatch.setattr(R, "_launch", plain_rotation)
+    plan = R.make_plan(8, 6, device="cpu")
+    pos = torch.tensor([0, 3, 70000, 5, 1])
+    return plan, pos, lambda x: plain_rotation(x, pos, plan, False, torch.empty_like(x))
+
+
+def test_rotate_carries_tangents(rotation):
+    plan, pos, want = rotation
+    x, t, g = (torch.randn(2, 3, 5, 8, dtype=torch.float32) for _ in range(3))
+    with fwd.dual_level():
+        for grad in (False, True):
+            dual = fwd.make_dual(x.clone().requires_grad_(grad), t)
+            y = fwd.unpack_dual(R.rotate(dual, pos, plan))
+            assert torch.equal(y.primal, want(x)) and torch.equal(y.tangent, want(t))
+        with torch.no_grad():                                   # no_grad stops gradients, not tangents
+            assert torch.equal(fwd.unpack_dual(R.rotate(dual, pos, plan)).tangent, want(t))
+        assert fwd.unpack_dual(R.rotate(x, pos, plan)).tangent is None
+        with pytest.raises(ValueError, match="gradient"):
+            R.rotate(fwd.make_dual(x, t), pos, plan, out=torch.empty_like(x))
+    with fwd.dual_level():                                      # forward over reverse: the gradient's tangent
+        x0 = x.clone().requires_grad_(True)
+        y = R.rotate(x0, pos, plan)
+        gx, = torch.autograd.grad(y, x0, fwd.make_dual(g, t), create_graph=True)
+        inv = lambda z: plain_rotation(z, pos, plan, True, torch.empty_like(z))          # noqa: E731
+        gx = fwd.unpack_dual(gx)
+        assert torch.equal(gx.primal, inv(g)) and torch.equal(gx.tangent, inv(t))
+
+
+def test_rotate_append_refuses_tangents(lib):
+    x, c = torch.randn(3, 2, 8), torch.zeros(2, 16, 2, 8)
+    plan, pos = R.make_plan(8, device="cpu"), torch.arange(3)
+    with fwd.dual_level():
+        for i in range(3):
+            qkv = [fwd.make_dual(x, x) if i == j else x for j in range(3)]
+            with pytest.raises(ValueError, match="gradient"):
+                R.rotate_append(*qkv, pos, pos, c, c.clone(), plan)
     assert not lib.names()
