@@ -239,8 +239,9 @@ def _check_lattice(q, kv, H, dh):
 
 
 def _check_out(out, shape, dev):
-    if out.shape != shape or out.device != dev or not _A._written_once(out):
-        raise ValueError("out must be %s on the query's device, with no shared elements" % (tuple(shape),))
+    if out.shape != shape or out.device != dev or not _A._written_once(out) or out.is_neg():
+        raise ValueError("out must be %s on the query's device, with no shared elements, and no negative view" %
+                         (tuple(shape),))
 
 
 def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtype=None, check=True):
@@ -259,6 +260,7 @@ def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtyp
     N, H, dh = q.shape
     B = kv.seq_lens.numel()
     dev, KVH = _check_lattice(q, kv, H, dh)
+    q = q.resolve_neg()
     _A._require_cuda(q, cu_q, *[t for t in (prefix_lens, active) if t is not None])
     if cu_q.shape != (B + 1,) or cu_q.dtype != torch.int32:
         raise ValueError("cu_q must be [%d] int32" % (B + 1))
@@ -311,6 +313,7 @@ def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
     if shared_len < 0:
         raise ValueError("shared_len must not be negative")
     dev, KVH = _check_lattice(q, kv, H, dh)
+    q = q.resolve_neg()
     if kv.seq_lens.shape[0] != B:
         raise ValueError("query does not match the lattice")
     if shared_len < KB:

@@ -86,6 +86,7 @@ def _launch(x, positions, plan, inverse, out):
     dev = _A._require_cuda(x, positions, plan.freq, out)
     if x.numel() == 0:
         return out
+    x = x.resolve_neg()                          # (gradients through the imaginary part of a conjugate come as views)
     x4, y4 = (x, out) if x.dim() == 4 else (x.transpose(0, 1)[None], out.transpose(0, 1)[None])
     B, H, T, dh = x4.shape
     ps = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
@@ -142,8 +143,8 @@ def rotate(x, positions, plan, inverse=False, out=None):
         return _launch(x, positions, plan, inverse, torch.empty_like(x))
     if out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("out must have x's shape and dtype")
-    if not _A._written_once(out):
-        raise ValueError("out has elements that share memory")
+    if not _A._written_once(out) or out.is_neg():
+        raise ValueError("out has elements that share memory, or is a negative view")
     return _launch(x, positions, plan, inverse, out)
 
 
@@ -156,6 +157,9 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
     dev = _A._require_cuda(query, key, value, positions, slot_mapping, k_cache, v_cache, plan.freq)
     if _A._differentiable(query, key, value):
         raise ValueError("rotate_append has no gradient (use rotate)")
+    query, key, value = query.resolve_neg(), key.resolve_neg(), value.resolve_neg()
+    if k_cache.is_neg() or v_cache.is_neg() or (out is not None and out.is_neg()):
+        raise ValueError("out and the caches must not be negative views")
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.device != dev:

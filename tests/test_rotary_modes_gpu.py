@@ -22,3 +22,13 @@ def test_tangents(layout, rot, dtype):
         wide = torch.randn(2, 9, 3, 65, device="cuda").to(dtype)[..., :64].transpose(1, 2)      # a strided tangent
         y = fwd.unpack_dual(R.rotate(fwd.make_dual(x, wide), pos, plan, inverse=True))
         assert torch.equal(y.tangent, R.rotate(wide, pos, plan, inverse=True))
+
+
+def test_gradients_that_arrive_as_negative_views():
+    plan, pos = R.make_plan(64), torch.arange(9, device="cuda")
+    x, zero = torch.randn(2, 3, 9, 64, device="cuda", requires_grad=True), torch.zeros(2, 3, 9, 64, device="cuda")
+    w = torch.randn(2, 3, 9, 64, device="cuda", dtype=torch.complex64)
+    torch.autograd.backward(torch.complex(zero, R.rotate(x, pos, plan)), w.conj())
+    assert torch.equal(x.grad, R.rotate((-w.imag).contiguous(), pos, plan, inverse=True))
+    view = w.conj().imag
+    assert view.is_neg() and torch.equal(R.rotate(view, pos, plan), R.rotate(view.clone(), pos, plan))

@@ -1,5 +1,7 @@
 """The host layer of the serving-step operators without a GPU: the library is a stand-in that records its calls, so what
 is tested is everything around the kernels (workspaces, checks, gradients, versions), on CPU tensors."""
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad as fwd
@@ -131,3 +133,41 @@ def test_rotate_append_refuses_tangents(lib):
             with pytest.raises(ValueError, match="gradient"):
                 R.rotate_append(*qkv, pos, pos, c, c.clone(), plan)
     assert not lib.names()
+
+
+def neg(x):
+    """-x as a negative view: x in memory, a bit that says the sign is the other one."""
+    y = torch.complex(torch.zeros_like(x), x).conj().imag
+    assert y.is_neg() and torch.equal(y, -x)
+    return y
+
+
+def test_negative_views_are_read_as_their_values(lib):
+    """The kernels read memory: a view whose sign is pending is resolved, as an input; written, it is refused."""
+    first = lambda t: t.reshape(-1)[0].item()                   # noqa: E731
+    plan, pos = R.make_plan(64, device="cpu"), torch.arange(3)
+    x, c = torch.randn(3, 2, 64), torch.zeros(2, 16, 2, 64)
+    kv, cu = lattice(), torch.tensor([0, 2, 3], dtype=torch.int32)
+    for n, call in ((3, lambda q, k, v: R.rotate_append(q, k, v, pos, pos, c, c.clone(), plan)),
+                    (1, lambda q, k, v: R.rotate(q, pos, plan)), (1, lambda q, k, v: D.decode_shared(q[:2], kv, 256)),
+                    (1, lambda q, k, v: D.prefill_paged(q, kv, cu))):
+        got, qkv = [], [neg(torch.randn(3, 2, 64)) for i in range(3)]
+        for name in ("lssab8_rotate", "lssab8_rotate_append", "lssab8_prefill_paged", "lssab8_decode_shared"):
+            setattr(lib, name, lambda *a: got.extend(ctypes.c_float.from_address(p).value for p in a[:n]) or 0)
+        call(*qkv)
+        assert got == [first(t) for t in qkv[:n]]
+    for call in (lambda o: R.rotate(x, pos, plan, out=o), lambda o: R.rotate_append(x, x, x, pos, pos, c, c, plan, out=o),
+                 lambda o: R.rotate_append(x, x, x, pos, pos, o, c, plan)):
+        with pytest.raises(ValueError, match="negative view"):
+            call(neg(torch.randn(3, 2, 64)))
+
+
+def test_gradients_that_arrive_as_negative_views(rotation, monkeypatch):
+    """The gradient of an imaginary part is a negative view of complex memory."""
+    plan, pos, _ = rotation
+    seen = []
+    monkeypatch.setattr(R, "_launch", lambda x, *a: seen.append(x.is_neg()) or plain_rotation(x, *a))
+    x, w = torch.randn(1, 1, 5, 8, requires_grad=True), torch.randn(1, 1, 5, 8, dtype=torch.complex64)
+    torch.autograd.backward(torch.complex(torch.zeros(1, 1, 5, 8), R.rotate(x, pos, plan)), w.conj())
+    assert seen == [False, True]                                # it does arrive so, and _launch resolves it (above)
+    assert torch.equal(x.grad, plain_rotation(-w.imag, pos, plan, True, torch.empty(1, 1, 5, 8)))
