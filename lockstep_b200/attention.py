@@ -69,6 +69,12 @@ def _differentiable(*ts):
     return _fwd._current_level >= 0 and any(_fwd.unpack_dual(t).tangent is not None for t in ts)
 
 
+def _wrote(*ts):
+    """The kernels write through pointers: raise the tensors' versions, so that autograd sees the change as it sees those
+    of torch's own in-place operators."""
+    torch.autograd.graph.increment_version(ts)
+
+
 def _require_cuda(*ts):
     for t in ts:
         if not isinstance(t, torch.Tensor) or not t.is_cuda:

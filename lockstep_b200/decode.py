@@ -242,6 +242,8 @@ def _check_out(out, shape, dev):
     if out.shape != shape or out.device != dev or not _A._written_once(out) or out.is_neg():
         raise ValueError("out must be %s on the query's device, with no shared elements, and no negative view" %
                          (tuple(shape),))
+    if _A._differentiable(out):
+        raise ValueError("out= has no gradient: give a tensor that requires none")
 
 
 def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtype=None, check=True):
@@ -268,7 +270,8 @@ def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtyp
         raise ValueError("prefix_lens must be [%d] int32" % B)
     if active is not None and (active.shape != (B,) or active.dtype != torch.bool):
         raise ValueError("active must be [%d] bool" % B)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
     else:
         _check_out(out, q.shape, dev)
@@ -292,6 +295,8 @@ def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtyp
             kv.num_pages, kv.k8p.data_ptr(), kv.v8p.data_ptr(), kv.ek.data_ptr(), kv.ev.data_ptr(), kv.ev0.data_ptr(),
             kv.max_blocks, int(kv.sink), out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64c(out.stride()),
             ws.data_ptr(), nbytes, _A._stream_handle(dev)), "lssab8_prefill_paged")
+    if not fresh:
+        _A._wrote(out)
     if check:
         _A.check_device_errors(dev)
     return out
@@ -317,12 +322,16 @@ def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
     if kv.seq_lens.shape[0] != B:
         raise ValueError("query does not match the lattice")
     if shared_len < KB:
-        if out is not None:
-            _check_out(out, q.shape, dev)
-        return decode(q, kv, out=out, out_dtype=out_dtype, check=check)
+        if out is None:
+            return decode(q, kv, out_dtype=out_dtype, check=check)
+        _check_out(out, q.shape, dev)
+        decode(q, kv, out=out, check=check)
+        _A._wrote(out)
+        return out
     if shared_len // KB > kv.max_blocks or shared_len // KB * (KB // PAGE) > kv.block_table.shape[1]:
         raise ValueError("the lattice holds at most %d blocks a sequence" % kv.max_blocks)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
     else:
         _check_out(out, q.shape, dev)
@@ -338,6 +347,8 @@ def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
             kv.v8p.data_ptr(), kv.ek.data_ptr(), kv.ev.data_ptr(), kv.ev0.data_ptr(), kv.max_blocks, int(kv.sink),
             out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64c(out.stride()), ws.data_ptr(), nbytes,
             _A._stream_handle(dev)), "lssab8_decode_shared")
+    if not fresh:
+        _A._wrote(out)
     if check:
         _A.check_device_errors(dev)
     return out

@@ -60,6 +60,7 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
     if not 0 <= cap < 1 << 31:
         raise ValueError("max_tokens must be from 0 to 2^31 - 1")
     lens, new_tokens, free_pages = lens.contiguous(), new_tokens.contiguous(), free_pages.contiguous()
+    wrote = [block_table]
     if out is None:
         out = alloc_step_tables(n, cap, dev)
     else:
@@ -68,6 +69,7 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
             t, w = getattr(out, f), getattr(want, f)
             if t.shape != w.shape or t.dtype != w.dtype or t.device != dev or not t.is_contiguous():
                 raise ValueError("out: tables of another step shape (%s)" % f)
+            wrote.append(t)
         if out.seq_lens.data_ptr() in (lens.data_ptr(), new_tokens.data_ptr()):
             raise ValueError("out.seq_lens must not be the step's own lens or new_tokens")
     with _A._on(dev):
@@ -76,6 +78,7 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
             free_pages.data_ptr() if nfree else None, nfree, cap,
             out.query_start_loc.data_ptr(), out.seq_lens.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(),
             out.seq_index.data_ptr(), out.pages_used.data_ptr(), _A._stream_handle(dev)), "lssab8_step_tables")
+    _A._wrote(*wrote)
     if check:
         _A.check_device_errors(dev)
     return out

@@ -145,7 +145,11 @@ def rotate(x, positions, plan, inverse=False, out=None):
         raise ValueError("out must have x's shape and dtype")
     if not _A._written_once(out) or out.is_neg():
         raise ValueError("out has elements that share memory, or is a negative view")
-    return _launch(x, positions, plan, inverse, out)
+    if _A._differentiable(out):
+        raise ValueError("out= has no gradient: rotate into a tensor that requires none")
+    _launch(x, positions, plan, inverse, out)
+    _A._wrote(out)
+    return out
 
 
 def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, plan, out=None, check=True):
@@ -158,9 +162,12 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
     if _A._differentiable(query, key, value):
         raise ValueError("rotate_append has no gradient (use rotate)")
     query, key, value = query.resolve_neg(), key.resolve_neg(), value.resolve_neg()
+    if _A._differentiable(k_cache, v_cache) or (out is not None and _A._differentiable(out)):
+        raise ValueError("rotate_append has no gradient: out and the caches must not require one")
     if k_cache.is_neg() or v_cache.is_neg() or (out is not None and out.is_neg()):
         raise ValueError("out and the caches must not be negative views")
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.device != dev:
         raise ValueError("out must be on the query's device")
@@ -178,6 +185,10 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
             positions.stride(0), plan.freq.data_ptr(), plan.factor, plan.rotary_dim, _LAYOUTS[plan.layout],
             out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), cdt, kcs, vcs, k_cache.shape[0],
             slot_mapping.data_ptr(), _A._stream_handle(dev)), "lssab8_rotate_append")
+    if fresh:
+        _A._wrote(k_cache, v_cache)
+    else:
+        _A._wrote(k_cache, v_cache, out)
     if check:
         _A.check_device_errors(dev)
     return out

@@ -32,3 +32,17 @@ def test_gradients_that_arrive_as_negative_views():
     assert torch.equal(x.grad, R.rotate((-w.imag).contiguous(), pos, plan, inverse=True))
     view = w.conj().imag
     assert view.is_neg() and torch.equal(R.rotate(view, pos, plan), R.rotate(view.clone(), pos, plan))
+
+
+def test_in_place_writes_are_seen_by_autograd():
+    plan, pos = R.make_plan(64), torch.arange(9, device="cuda")
+    x, w = torch.randn(9, 3, 64, device="cuda"), torch.randn(9, 3, 64, device="cuda", requires_grad=True)
+    y = (w * x).sum()
+    R.rotate(x, pos, plan, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():                                # where torch keeps no versions
+        z = torch.randn(9, 3, 64, device="cuda")
+        want = R.rotate(z, pos, plan)
+        assert torch.equal(R.rotate(z, pos, plan, out=z), want)
+    assert torch.equal(R.rotate(z, pos, plan, out=z), R.rotate(want, pos, plan))

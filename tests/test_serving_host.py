@@ -9,6 +9,7 @@ from torch.autograd import forward_ad as fwd
 from lockstep_b200 import _lib
 from lockstep_b200 import attention as A
 from lockstep_b200 import decode as D
+from lockstep_b200 import paging as P
 from lockstep_b200 import rotary as R
 
 
@@ -171,3 +172,55 @@ def test_gradients_that_arrive_as_negative_views(rotation, monkeypatch):
     torch.autograd.backward(torch.complex(torch.zeros(1, 1, 5, 8), R.rotate(x, pos, plan)), w.conj())
     assert seen == [False, True]                                # it does arrive so, and _launch resolves it (above)
     assert torch.equal(x.grad, plain_rotation(-w.imag, pos, plan, True, torch.empty(1, 1, 5, 8)))
+
+
+def version_of(*ts):
+    return [t._version for t in ts]
+
+
+def test_writes_raise_versions(lib):
+    """What a kernel writes in place, autograd sees: a tensor saved for a backward pass and rewritten raises there."""
+    plan, pos = R.make_plan(64, device="cpu"), torch.arange(3)
+    x, kc, vc = torch.randn(3, 2, 64), torch.zeros(2, 16, 2, 64), torch.zeros(2, 16, 2, 64)
+    kv, cu = lattice(), torch.tensor([0, 2, 3], dtype=torch.int32)
+    i32 = torch.zeros(2, dtype=torch.int32)
+    t, bt = P.alloc_step_tables(2, 3, "cpu"), torch.zeros(2, 4, dtype=torch.int32)
+    fields = [getattr(t, f) for f in P.StepTables.__dataclass_fields__]
+    q = torch.randn(3, 4, 64)
+    for ts, call in (([x], lambda: R.rotate(x, pos, plan, out=x)),
+                     ([x, kc, vc], lambda: R.rotate_append(x, x.clone(), x.clone(), pos, pos, kc, vc, plan, out=x)),
+                     ([kc, vc], lambda: R.rotate_append(x, x.clone(), x.clone(), pos, pos, kc, vc, plan)),
+                     ([q], lambda: D.prefill_paged(q.clone(), kv, cu, out=q)),
+                     ([q], lambda: D.decode_shared(q[:2].clone(), kv, 256, out=q[:2])),
+                     ([q], lambda: D.decode_shared(q[:2].clone(), kv, 100, out=q[:2])),
+                     ([bt] + fields, lambda: P.step_tables(i32, i32.clone(), bt, i32, 3, out=t)),
+                     ([bt], lambda: P.step_tables(i32, i32.clone(), bt, i32, 3))):
+        before = version_of(*ts)
+        call()
+        assert all(a > b for a, b in zip(version_of(*ts), before))
+    keep = version_of(x, q)
+    R.rotate(x, pos, plan)
+    D.prefill_paged(q, kv, cu)
+    assert version_of(x, q) == keep                             # what is only read keeps its version
+    w = torch.randn(3, 2, 64, requires_grad=True)
+    y = (w * x).sum()
+    R.rotate(x, pos, plan, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_outputs_that_require_a_gradient_are_refused(lib):
+    plan, pos = R.make_plan(64, device="cpu"), torch.arange(3)
+    x, c = torch.randn(3, 2, 64), torch.zeros(2, 16, 2, 64)
+    kv, cu = lattice(), torch.tensor([0, 2, 3], dtype=torch.int32)
+    leaf = lambda *s: torch.zeros(s, requires_grad=True)        # noqa: E731
+    for call in (lambda: R.rotate(x, pos, plan, out=leaf(3, 2, 64)),
+                 lambda: R.rotate_append(x, x, x, pos, pos, c, c.clone(), plan, out=leaf(3, 2, 64)),
+                 lambda: R.rotate_append(x, x, x, pos, pos, c, leaf(2, 16, 2, 64), plan),
+                 lambda: D.prefill_paged(x, kv, cu, out=leaf(3, 2, 64)),
+                 lambda: D.decode_shared(x[:2], kv, 256, out=leaf(2, 2, 64)),
+                 lambda: D.decode_shared(x[:2], kv, 100, out=leaf(2, 2, 64))):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():                                   # as torch's own out=
+            call()
