@@ -62,6 +62,57 @@ def _written_once(t):
     return _apart(t.stride(), t.shape)
 
 
+def _reach(strides, shape, dtype):
+    """(bytes from a tensor's first element to the end of its last, its dimensions as (stride in bytes, count))."""
+    size = dtype.itemsize
+    dims = tuple((st * size, n) for st, n in zip(strides, shape) if n != 1)
+    return sum((n - 1) * st for st, n in dims) + size if all(shape) else 0, dims + ((1, size),)
+
+
+@functools.lru_cache(maxsize=4096)
+def _meet(delta, a, b):
+    """Whether byte sets a and b, ((stride, count), ...) each, share a byte when b starts delta bytes after a: delta =
+    sum of i_k s_k over a's dimensions less the same over b's.  Strides of both sides taken together, largest first, each
+    tried only where the smaller ones can make up the rest; a search that grows past 100,000 steps counts as shared."""
+    span = {}
+    for dims, sign in ((a, 1), (b, -1)):
+        for st, n in dims:
+            lo, hi = span.get(st, (0, 0))
+            span[st] = (lo - (n - 1), hi) if sign < 0 else (lo, hi + n - 1)
+    terms = [(st, *span[st]) for st in sorted((st for st in span if st), reverse=True)]
+    rest = [(0, 0)]                                  # what the terms after each can reach
+    for st, lo, hi in reversed(terms):
+        rest.append((rest[-1][0] + st * lo, rest[-1][1] + st * hi))
+    rest.reverse()
+    steps = 0
+
+    def reach(k, d):
+        nonlocal steps
+        steps += 1
+        if steps > 100000:
+            return True
+        if k == len(terms):
+            return d == 0
+        st, lo, hi = terms[k]
+        rlo, rhi = rest[k + 1]
+        return any(reach(k + 1, d - st * i) for i in range(max(lo, -((rhi - d) // st)), min(hi, (d - rlo) // st) + 1))
+
+    return reach(0, delta)
+
+
+def _share(a, b):
+    """Whether tensors a and b share memory."""
+    (na, da), (nb, db) = _reach(a.stride(), a.shape, a.dtype), _reach(b.stride(), b.shape, b.dtype)
+    delta = b.data_ptr() - a.data_ptr()
+    return -nb < delta < na and na * nb > 0 and _meet(delta, da, db)
+
+
+def _same_places(a, b):
+    """Whether a and b are the same elements in the same places."""
+    return a.data_ptr() == b.data_ptr() and a.dtype == b.dtype and a.shape == b.shape and all(
+        x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n > 1)
+
+
 def _differentiable(*ts):
     """A derivative would have to flow through one of ts: it requires a gradient, or carries a forward-mode tangent."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in ts):

@@ -147,6 +147,8 @@ def rotate(x, positions, plan, inverse=False, out=None):
         raise ValueError("out has elements that share memory, or is a negative view")
     if _A._differentiable(out):
         raise ValueError("out= has no gradient: rotate into a tensor that requires none")
+    if not _A._same_places(x, out) and _A._share(x, out):
+        raise ValueError("out must be x itself or lie apart from it")
     _launch(x, positions, plan, inverse, out)
     _A._wrote(out)
     return out
@@ -175,9 +177,11 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
                         value.stride(), value.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape,
                         v_cache.stride(), v_cache.dtype, out.shape, out.stride(), out.dtype, positions.shape,
                         positions.dtype, slot_mapping.shape, slot_mapping.dtype, plan.head_dim)
-    dims, qs, ks, vs, pos64, os_, cdt, kcs, vcs = args
+    dims, qs, ks, vs, pos64, os_, cdt, kcs, vcs, in_place, places = args
     if dims[1] == 0:
         return out
+    _check_places(tuple(zip((query.data_ptr(), key.data_ptr(), value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                             out.data_ptr()), places)), in_place)
     slot_mapping = slot_mapping.contiguous()
     with _A._on(dev):
         _lib.check(_lib.load().lssab8_rotate_append(
@@ -222,4 +226,20 @@ def _append_args(q, qst, qdt, k, kst, kdt, v, vst, vdt, kc, kcst, kcdt, vc, vcst
     if not (_A._apart(ost, o) and _A._apart(kcst, kc) and _A._apart(vcst, vc)):
         raise ValueError("out and the caches must not have elements that share memory")
     return ((_A.dtype_code(qdt), N, H, KVH, dh), _lib.i64c(qst[:2]), _lib.i64c(kst[:2]), _lib.i64c(vst[:2]),
-            int(pdt == torch.int64), _lib.i64c(ost[:2]), _A.dtype_code(kcdt), _lib.i64c(kcst[:3]), _lib.i64c(vcst[:3]))
+            int(pdt == torch.int64), _lib.i64c(ost[:2]), _A.dtype_code(kcdt), _lib.i64c(kcst[:3]), _lib.i64c(vcst[:3]),
+            all(x == y for x, y, n in zip(qst, ost, q) if n > 1),
+            tuple(_A._reach(*x) for x in ((qst, q, qdt), (kst, k, kdt), (vst, v, vdt), (kcst, kc, kcdt), (vcst, vc, vcdt),
+                                          (ost, o, odt))))
+
+
+def _check_places(at, in_place):
+    """What rotate_append writes (caches, out) lies apart from what it reads, except out on the query itself, and from
+    each other; at: (address, (bytes reached, its dimensions)) of query, key, value, caches, out."""
+    reads, writes = at[:3], at[3:]
+    lo, hi = min(p for p, _ in reads), max(p + n for p, (n, _) in reads)
+    for i, (p, (n, dims)) in enumerate(writes):
+        for j, (p2, (n2, dims2)) in enumerate(writes[:i] + (reads if p < hi and lo < p + n else ())):
+            if p < p2 + n2 and p2 < p + n and not (i == 2 and j == 2 and in_place and p == p2) and \
+                    _A._meet(p2 - p, dims, dims2):
+                raise ValueError("out and the caches must lie apart from the inputs (out may be the query itself) and from "
+                                 "each other")

@@ -1,6 +1,8 @@
 """The host layer of the serving-step operators without a GPU: the library is a stand-in that records its calls, so what
 is tested is everything around the kernels (workspaces, checks, gradients, versions), on CPU tensors."""
 import ctypes
+import itertools
+import random
 
 import pytest
 import torch
@@ -224,3 +226,53 @@ def test_outputs_that_require_a_gradient_are_refused(lib):
             call()
         with torch.no_grad():                                   # as torch's own out=
             call()
+
+
+def test_shared_memory_is_found_exactly():
+    r = random.Random(3)
+    buf, found = torch.zeros(1000), [0, 0]
+
+    def draw():
+        n = r.randint(1, 4)
+        shape, stride = [r.randint(1, 4) for _ in range(n)], [r.choice([0, 1, 2, 3, 4, 5, 6, 8, 12, 24]) for _ in range(n)]
+        return torch.as_strided(buf.view(r.choice([torch.float32, torch.float16])), shape, stride, r.randint(0, 60))
+
+    def places(t):
+        return {t.data_ptr() + sum(i * s for i, s in zip(ix, t.stride())) * t.element_size() + b
+                for ix in itertools.product(*map(range, t.shape)) for b in range(t.element_size())}
+    for _ in range(1500):
+        a, b = draw(), draw()
+        want = bool(places(a) & places(b))
+        found[want] += 1
+        assert A._share(a, b) == want, (a.shape, a.stride(), b.shape, b.stride())
+    assert min(found) > 300 and not A._share(buf[:0], buf) and not A._share(buf, torch.zeros(1000))
+
+
+def test_outputs_over_other_inputs_are_refused(lib):
+    plan, pos = R.make_plan(64, device="cpu"), torch.arange(3)
+    wide = torch.randn(4, 2, 130)
+    x = wide[:3, :, :64]
+    for out in (x, wide[:3, :, 64:128], torch.empty(3, 2, 64)):          # itself, between its rows, elsewhere
+        R.rotate(x, pos, plan, out=out)
+    buf = torch.randn(400)
+    for a, out in ((x, wide[1:, :, :64]), (x, wide[:3, :, 1:65]), (buf[:384].view(3, 2, 64), buf[1:385].view(3, 2, 64)),
+                   (wide[:3, :, :64], wide.view(-1)[2:].as_strided((3, 2, 64), (260, 130, 1)))):
+        with pytest.raises(ValueError, match="apart"):
+            R.rotate(a, pos, plan, out=out)
+    del lib.calls[:]
+    qkv = torch.randn(3, 6, 64)                                          # one projection, cut
+    q, k, v = qkv[:, :2], qkv[:, 2:4], qkv[:, 4:]
+    c = torch.zeros(4, 2, 16, 2, 64)                                     # one cache, keys and values page by page
+    go = lambda out=None, kc=c[:, 0], vc=c[:, 1]: R.rotate_append(q, k, v, pos, pos, kc, vc, plan, out=out)   # noqa: E731
+    for out in (None, q, torch.empty(3, 2, 64)):
+        go(out)
+    n = len(lib.names())
+    for kw in (dict(out=k), dict(out=v), dict(out=qkv[:, 1:3]), dict(out=c[0, 0, :3]), dict(vc=c[:, 0]),
+               dict(kc=torch.zeros(4, 16, 2, 64), vc=c[:, 0], out=c[3, 0, 13:]),
+               dict(vc=c.view(-1)[1:].as_strided((4, 16, 2, 64), (4096, 128, 64, 1)))):
+        with pytest.raises(ValueError, match="apart"):
+            go(**kw)
+    store = torch.zeros(2, 16, 2, 64)                                    # keys that lie in the cache they go to
+    with pytest.raises(ValueError, match="apart"):
+        R.rotate_append(q, store[1, :3], v, pos, pos, store, c[:2, 1], plan)
+    assert len(lib.names()) == n
