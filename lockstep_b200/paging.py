@@ -70,8 +70,11 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
             if t.shape != w.shape or t.dtype != w.dtype or t.device != dev or not t.is_contiguous():
                 raise ValueError("out: tables of another step shape (%s)" % f)
             wrote.append(t)
-        if out.seq_lens.data_ptr() in (lens.data_ptr(), new_tokens.data_ptr()):
-            raise ValueError("out.seq_lens must not be the step's own lens or new_tokens")
+        ins = [(x.data_ptr(), x.data_ptr() + 4 * size, x) for x, size in (
+            (lens, n), (new_tokens, n), (block_table, (n - 1) * pitch + width), (free_pages, nfree))]
+        outs = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), t) for t in wrote[1:]]
+        if any(p < e2 and p2 < e and _A._share(t, x) for p, e, t in outs for p2, e2, x in ins):
+            raise ValueError("out must lie apart from the step's own lengths, table and free pages")
     with _A._on(dev):
         _lib.check(_lib.load().lssab8_step_tables(
             lens.data_ptr(), new_tokens.data_ptr(), n, block_table.data_ptr(), max(pitch, width), width,

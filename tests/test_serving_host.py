@@ -276,3 +276,21 @@ def test_outputs_over_other_inputs_are_refused(lib):
     with pytest.raises(ValueError, match="apart"):
         R.rotate_append(q, store[1, :3], v, pos, pos, store, c[:2, 1], plan)
     assert len(lib.names()) == n
+
+
+def test_tables_over_their_inputs_are_refused(lib):
+    """Every CTA of the kernel reads all lengths while the first writes the new ones."""
+    buf = torch.zeros(64, dtype=torch.int32)
+    lens, new, free, bt = buf[0:4], buf[8:12], buf[16:20], buf[24:40].view(4, 4)
+    t = P.alloc_step_tables(4, 3, "cpu")
+    P.step_tables(lens, new, bt, free, 3, out=t)
+    for at in (1, 3, 9, 11, 17, 25, 39):
+        for name, n in (("seq_lens", 4), ("query_start_loc", 5), ("pages_used", 1)):
+            u = P.alloc_step_tables(4, 3, "cpu")
+            setattr(u, name, buf[at:at + n])
+            with pytest.raises(ValueError):
+                P.step_tables(lens, new, bt, free, 3, out=u)
+    u = P.alloc_step_tables(4, 3, "cpu")
+    u.seq_lens = buf[4:8]                                       # next to the lengths, not over them
+    P.step_tables(lens, new, bt, free, 3, out=u)
+    assert lib.names() == ["lssab8_step_tables"] * 2
