@@ -235,6 +235,8 @@ def _check_lattice(q, kv, H, dh):
     i32 = torch.int32
     if lens.dtype != i32 or table.dtype != i32 or ek.dtype != i32 or ev.dtype != i32 or ev0.dtype != i32:
         raise TypeError("the lattice's lengths, table and exponents must be int32")
+    if k8p.dtype != torch.int8 or v8p.dtype != torch.int8:
+        raise TypeError("the lattice's pages must be int8")
     return dev, k8p.shape[1]
 
 

@@ -294,3 +294,16 @@ def test_tables_over_their_inputs_are_refused(lib):
     u.seq_lens = buf[4:8]                                       # next to the lengths, not over them
     P.step_tables(lens, new, bt, free, 3, out=u)
     assert lib.names() == ["lssab8_step_tables"] * 2
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.bfloat16, torch.float32, torch.float8_e4m3fn])
+@pytest.mark.parametrize("pool", ["k8p", "v8p"])
+def test_page_pools_of_another_type_are_refused(lib, pool, dtype):
+    kv = lattice()
+    setattr(kv, pool, getattr(kv, pool).to(dtype))
+    for call in (lambda: D.prefill_paged(torch.zeros(3, 4, 64), kv, torch.tensor([0, 2, 3], dtype=torch.int32)),
+                 lambda: D.decode_shared(torch.zeros(2, 4, 64), kv, 256),
+                 lambda: D.decode_shared(torch.zeros(2, 4, 64), kv, 0)):
+        with pytest.raises(TypeError, match="int8"):
+            call()
+    assert not lib.names()
