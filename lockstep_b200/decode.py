@@ -258,12 +258,14 @@ def prefill_paged(q, kv, cu_q, prefix_lens=None, active=None, out=None, out_dtyp
     that is farther (prefix mask).  Without a prefix every row is bit-identical to the prefill of its sequence
     alone.  active [B] bool: the sequences that have rows here (None: all); other rows of out, and rows outside
     cu_q, stay as they were (a new out: undefined).  Lengths that break these rules raise RuntimeError
-    (device error 16) when checked."""
+    (device error 16) when checked.  Inference only: a query that requires a gradient is refused."""
     if q.dim() != 3:
         raise ValueError("q must be [N, H, dh]")
     N, H, dh = q.shape
     B = kv.seq_lens.numel()
     dev, KVH = _check_lattice(q, kv, H, dh)
+    if _A._differentiable(q):
+        raise ValueError("prefill_paged has no gradient: give it a detached query")
     q = q.resolve_neg()
     _A._require_cuda(q, cu_q, *[t for t in (prefix_lens, active) if t is not None])
     if cu_q.shape != (B + 1,) or cu_q.dtype != torch.int32:
@@ -312,7 +314,7 @@ def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
     (length > 0); they are read and scored once for the batch instead of once a sequence.  Fewer than 128
     shared tokens run decode.  A sequence that is shorter than the shared blocks, or does not hold the same
     ones, raises RuntimeError (device error 16) when checked.  Batches with several prefixes: one call for
-    each."""
+    each.  Inference only: a query that requires a gradient is refused."""
     if q.dim() != 3:
         raise ValueError("q must be [B, H, dh]")
     B, H, dh = q.shape
@@ -320,6 +322,8 @@ def decode_shared(q, kv, shared_len, out=None, out_dtype=None, check=True):
     if shared_len < 0:
         raise ValueError("shared_len must not be negative")
     dev, KVH = _check_lattice(q, kv, H, dh)
+    if _A._differentiable(q):
+        raise ValueError("decode_shared has no gradient: give it a detached query")
     q = q.resolve_neg()
     if kv.seq_lens.shape[0] != B:
         raise ValueError("query does not match the lattice")

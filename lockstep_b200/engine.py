@@ -204,6 +204,7 @@ class Lssab8Attention:
         if any(prompts):
             cu = torch.tensor(qsl, dtype=torch.int32, device=dev)
             act = torch.tensor(prompts, dtype=torch.bool, device=dev)
+            query = query.detach()                        # (the contract's integers have no gradient)
             if out.dtype == query.dtype:
                 D.prefill_paged(query, kv, cu, active=act, out=out)
             else:

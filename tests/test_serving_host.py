@@ -11,6 +11,7 @@ from torch.autograd import forward_ad as fwd
 from lockstep_b200 import _lib
 from lockstep_b200 import attention as A
 from lockstep_b200 import decode as D
+from lockstep_b200 import engine as E
 from lockstep_b200 import paging as P
 from lockstep_b200 import rotary as R
 
@@ -307,3 +308,32 @@ def test_page_pools_of_another_type_are_refused(lib, pool, dtype):
         with pytest.raises(TypeError, match="int8"):
             call()
     assert not lib.names()
+
+
+def test_attention_refuses_queries_with_a_gradient(lib):
+    kv, cu = lattice(), torch.tensor([0, 2, 3], dtype=torch.int32)
+    q = torch.randn(3, 4, 64)
+    calls = (lambda x: D.prefill_paged(x, kv, cu), lambda x: D.decode_shared(x[:2], kv, 256),
+             lambda x: D.decode_shared(x[:2], kv, 5))
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call(q.clone().requires_grad_(True))
+        with fwd.dual_level(), pytest.raises(ValueError, match="gradient"):
+            call(fwd.make_dual(q, q))
+        assert not lib.names()
+        with torch.no_grad():
+            call(q.clone().requires_grad_(True))
+        call(q)
+        del lib.calls[:]
+
+
+@pytest.mark.parametrize("prefill", [True, False])
+def test_engine_takes_projections_that_require_a_gradient(lib, prefill):
+    """An engine in a program that records gradients: its attention is cut off from them, as ever."""
+    att = E.Lssab8Attention(4, 2, 64, 40, max_len=512, max_seqs=2, device="cpu")
+    c = torch.zeros(2, 40, 16, 2, 64)
+    table = torch.arange(32, dtype=torch.int32)[None]
+    meta = E.StepMeta([0, 1], [1], table, torch.zeros(1, dtype=torch.long), [prefill])
+    q, k, v = (torch.randn(1, h, 64, requires_grad=True) for h in (4, 2, 2))
+    out = att.forward(0, q, k.detach(), v.detach(), c[0], c[1], meta)
+    assert not out.requires_grad and lib.names()[-1] == ("lssab8_prefill_paged" if prefill else "lssab8_decode")
