@@ -205,10 +205,11 @@ class Lssab8Attention:
             cu = torch.tensor(qsl, dtype=torch.int32, device=dev)
             act = torch.tensor(prompts, dtype=torch.bool, device=dev)
             query = query.detach()                        # (the contract's integers have no gradient)
+            q = query[:qsl[-1]]                           # (query and out may be longer than the step's rows)
             if out.dtype == query.dtype:
-                D.prefill_paged(query, kv, cu, active=act, out=out)
+                D.prefill_paged(q, kv, cu, active=act, out=out[:qsl[-1]])
             else:
-                rows = D.prefill_paged(query, kv, cu, active=act)
+                rows = D.prefill_paged(q, kv, cu, active=act)
                 for i in range(nseq):
                     if prompts[i]:
                         out[qsl[i]:qsl[i + 1]] = rows[qsl[i]:qsl[i + 1]]

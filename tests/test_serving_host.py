@@ -337,3 +337,14 @@ def test_engine_takes_projections_that_require_a_gradient(lib, prefill):
     q, k, v = (torch.randn(1, h, 64, requires_grad=True) for h in (4, 2, 2))
     out = att.forward(0, q, k.detach(), v.detach(), c[0], c[1], meta)
     assert not out.requires_grad and lib.names()[-1] == ("lssab8_prefill_paged" if prefill else "lssab8_decode")
+
+
+@pytest.mark.parametrize("nq,nout", [(3, 8), (8, 3), (8, 8), (6, 9)])
+def test_engine_takes_buffers_longer_than_the_step(lib, nq, nout):
+    att = E.Lssab8Attention(4, 2, 64, 40, max_len=512, max_seqs=2, device="cpu")
+    c, table = torch.zeros(2, 40, 16, 2, 64), torch.arange(64, dtype=torch.int32).view(2, 32)
+    meta = E.StepMeta([0, 2, 3], [2, 1], table, torch.tensor([0, 1, 512]), [True, False])
+    out = torch.zeros(nout, 4, 64)
+    att.forward(0, torch.randn(nq, 4, 64), torch.randn(3, 2, 64), torch.randn(3, 2, 64), c[0], c[1], meta, out=out)
+    (_, args), = [x for x in lib.calls if x[0] == "lssab8_prefill_paged"]
+    assert args[3] == 3 and args[22] == out.data_ptr()
