@@ -103,7 +103,13 @@ class LatticeLayer:
         the step is 0) takes a free slot, or the least recently used one of a sequence not in this
         step (an engine that never calls release() reuses its finished sequences' slots this way).
         A sequence that continues (length before > 0) must still hold its slot: if it was taken,
-        its block exponents are gone and the step is refused."""
+        its block exponents are gone and the step is refused.  So is one that continues past what
+        its slot holds, and a step in which two sequences start on one page (forks of a prompt that
+        share its pages): they would keep their exponents in one slot."""
+        if len(set(first_pages)) != len(first_pages):
+            twice = next(fp for i, fp in enumerate(first_pages) if fp in first_pages[:i])
+            raise RuntimeError("two sequences of the step start on page %d: sequences that share pages keep their own "
+                               "lattice and decode with decode_shared" % twice)
         self.step += 1
         out = []
         for fp, l0 in zip(first_pages, lens_before):
@@ -114,6 +120,9 @@ class LatticeLayer:
                                        "slot was reused (more live sequences than slots)" % (fp, l0))
                 s = self._take_slot()
                 self.slot_of[fp] = s
+            elif l0 > self.lens[s]:
+                raise RuntimeError("the sequence with first page %d continues at length %d, but its lattice holds %d "
+                                   "tokens" % (fp, l0, self.lens[s]))
             if l0 == 0:
                 self.lens[s] = 0                          # a new sequence (possibly on a reused first page)
             self.last_use[s] = self.step
@@ -185,16 +194,24 @@ class Lssab8Attention:
             bt = torch.cat([bt, bt.new_full((nseq, st.max_pages - bt.shape[1]), -1)], 1)
         bt = bt[:, :st.max_pages].contiguous()
         first = [int(x) for x in bt[:, 0].tolist()]
-        slots = st.slots(first, before)
-        sidx = torch.tensor(slots, dtype=torch.long, device=dev)
+        held = [i for i in range(nseq) if lens[i] > 0]     # (an idle row has no slot: its first page may be anyone's)
+        slots = st.slots([first[i] for i in held], [before[i] for i in held])
+        rows = [0] * nseq
+        for i, s in zip(held, slots):
+            rows[i] = s
+        sidx = torch.tensor(rows, dtype=torch.long, device=dev)
         kv = D.PagedKV(k8p=st.k8p, v8p=st.v8p, ek=st.ek[sidx].contiguous(), ev=st.ev[sidx].contiguous(),
                        ev0=st.ev0[sidx].contiguous(), block_table=bt,
                        seq_lens=torch.tensor(before, dtype=torch.int32, device=dev), max_blocks=st.max_blocks,
                        num_pages=st.num_pages, sink=self.sink)
         D.append_kv(kv, k_cache, v_cache, torch.tensor(lens, dtype=torch.int32, device=dev), src_block_table=bt)
-        st.ek[sidx], st.ev[sidx], st.ev0[sidx] = kv.ek, kv.ev, kv.ev0
-        for s, L in zip(slots, lens):
-            st.lens[s] = L
+        if len(held) == nseq:
+            st.ek[sidx], st.ev[sidx], st.ev0[sidx] = kv.ek, kv.ev, kv.ev0
+        else:
+            hi = torch.tensor(held, dtype=torch.long, device=dev)
+            st.ek[sidx[hi]], st.ev[sidx[hi]], st.ev0[sidx[hi]] = kv.ek[hi], kv.ev[hi], kv.ev0[hi]
+        for i, s in zip(held, slots):
+            st.lens[s] = lens[i]
         # 3. prompt rows: every sequence's block-aligned chunk in one packed prefill over the lattice
         prompts = [bool(meta.is_prefill[i]) and qlen[i] > 0 for i in range(nseq)]
         for i in range(nseq):

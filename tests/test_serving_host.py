@@ -348,3 +348,38 @@ def test_engine_takes_buffers_longer_than_the_step(lib, nq, nout):
     att.forward(0, torch.randn(nq, 4, 64), torch.randn(3, 2, 64), torch.randn(3, 2, 64), c[0], c[1], meta, out=out)
     (_, args), = [x for x in lib.calls if x[0] == "lssab8_prefill_paged"]
     assert args[3] == 3 and args[22] == out.data_ptr()
+
+
+def test_sequences_on_one_first_page_are_refused(lib):
+    """Lattice slots are kept by first page: forks would take one slot, an idle row takes none."""
+    att = E.Lssab8Attention(4, 2, 64, 40, max_len=512, max_seqs=3, device="cpu")
+    st, c = att.layers[0], torch.zeros(2, 40, 16, 2, 64)
+
+    def step(first, before, new):
+        table = torch.full((len(first), 4), -1, dtype=torch.int32)
+        table[:, 0] = torch.tensor(first, dtype=torch.int32)
+        qsl = [sum(new[:i]) for i in range(len(new) + 1)]
+        n = qsl[-1]
+        meta = E.StepMeta(qsl, [a + b for a, b in zip(before, new)], table, torch.zeros(n, dtype=torch.long),
+                          [x == 0 for x in before])
+        lib.lssab8_kv_append = lambda *a: att_exponents(a) or 0
+        att.forward(0, torch.randn(n, 4, 64), torch.randn(n, 2, 64), torch.randn(n, 2, 64), c[0], c[1], meta)
+
+    def att_exponents(args):                                    # the append writes its sequences' exponents
+        n = args[3]
+        ek = (ctypes.c_int32 * (n * 2 * st.max_blocks)).from_address(args[20])
+        for b in range(n):
+            ek[b * 2 * st.max_blocks] += 1
+
+    step([5, 9], [0, 0], [1, 1])
+    assert st.ek[st.slot_of[5], 0, 0] == 1 and st.ek[st.slot_of[9], 0, 0] == 1
+    with pytest.raises(RuntimeError, match="start on page 5"):
+        step([5, 5], [1, 1], [1, 1])
+    with pytest.raises(RuntimeError, match="start on page 7"):
+        step([7, 9, 7], [0, 1, 0], [1, 1, 1])
+    with pytest.raises(RuntimeError, match="holds 1 tokens"):
+        step([5], [2], [1])
+    keep = dict(st.slot_of)
+    step([5, -1, 9, -1, 5], [1, 0, 1, 0, 0], [1, 0, 1, 0, 0])   # idle rows, one over a live sequence's first page
+    assert st.slot_of == keep and st.lens[keep[5]] == st.lens[keep[9]] == 2
+    assert st.ek[keep[5], 0, 0] == 2 and st.ek[keep[9], 0, 0] == 2 and int((st.ek != 0).sum()) == 2
