@@ -39,6 +39,11 @@ enum : int {
   kDevPlan = 16,          // request lengths that do not fit their buffers, or sequences that do not share a prefix
 };
 
+// 128-key blocks and 16-token pages of a length, rounded up; right up to 2^31 - 1, where len + 127 would wrap and
+// pass for a length that fits (a length below 0 has none).
+__host__ __device__ constexpr int blocks_of(int len) { return len > 0 ? (len >> 7) + ((len & 127) != 0) : 0; }
+__host__ __device__ constexpr int pages_of(int len) { return len > 0 ? (len >> 4) + ((len & 15) != 0) : 0; }
+
 // dtype codes used across the C ABI
 enum : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
 

@@ -81,7 +81,7 @@ template <int DH, bool SINK, typename OutT, int kBatch>
 __device__ __forceinline__ void decode_merge_head(const DecodeArgs& p, int b, int g, int h, int c) {
   const int gq = p.group;
   const int L_len = p.seq_lens[b];
-  const int nblk = (L_len + kKB - 1) / kKB;
+  const int nblk = blocks_of(L_len);
   const long long bg = (long long)b * p.KVH + g;
   int v0c = 0, evs0 = 0, eh0 = 0;
   if (SINK && L_len > 1) {
@@ -160,7 +160,7 @@ decode_kernel(const DecodeArgs p) {
   const int split = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
   const int gq = p.group;
   const int L_len = p.seq_lens[b];
-  const int nblk = (L_len + kKB - 1) / kKB;
+  const int nblk = blocks_of(L_len);
   const int first = SHARED ? p.skip_blocks : 0;
   const int nsplit = (nblk - first + p.split_blocks - 1) / p.split_blocks;
   if (SHARED) pdl_launch_dependents();
@@ -168,7 +168,7 @@ decode_kernel(const DecodeArgs p) {
     if (SHARED) pdl_wait();
     return;
   }
-  if (nblk > p.max_blocks || (L_len + 15) / 16 > p.max_pages) {   // lattice arrays too short
+  if (nblk > p.max_blocks || pages_of(L_len) > p.max_pages) {   // lattice arrays too short
     if (tid == 0) atomicOr(p.err, kDevBadPage);
     if (SHARED) pdl_wait();
     return;
@@ -352,9 +352,9 @@ decode_prep_kernel(const InT* __restrict__ ksrc, const InT* __restrict__ vsrc, c
                    int32_t* __restrict__ ev0, int* __restrict__ err) {
   const int blk = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
   const int L_len = seq_lens[b];
-  const int nblk = (L_len + kKB - 1) / kKB;
+  const int nblk = blocks_of(L_len);
   if (blk >= nblk) return;
-  if (nblk > max_blocks || (L_len + 15) / 16 > max_pages) {        // lattice arrays too short
+  if (nblk > max_blocks || pages_of(L_len) > max_pages) {        // lattice arrays too short
     if (threadIdx.x == 0) atomicOr(err, kDevBadPage);
     return;
   }
@@ -494,16 +494,16 @@ kv_lattice_kernel(const InT* __restrict__ ksrc, const InT* __restrict__ vsrc, co
   const int blk = blockIdx.x, g = blockIdx.y, b = blockIdx.z >> 1;
   const bool isv = (blockIdx.z & 1) != 0;                // this CTA's tensor: K (0) or V (1)
   const int L = seq_lens[b];
-  const int nblk = (L + kKB - 1) / kKB;
+  const int nblk = blocks_of(L);
   if (blk >= nblk) return;
-  if (nblk > max_blocks || (L + 15) / 16 > max_pages) {
+  if (nblk > max_blocks || pages_of(L) > max_pages) {
     if (threadIdx.x == 0 && !isv) atomicOr(err, kDevBadPage);
     return;
   }
   if (start_lens && blk < start_lens[b] / kKB) return;   // complete before this append: unchanged
   const int pl = threadIdx.x / VPR, cv = threadIdx.x % VPR;
   const int lo = blk * kKB + pl * 16;                    // this thread's first key
-  const int npages = min(8, ((L + 15) / 16) - blk * 8);  // pages of this block that exist
+  const int npages = min(8, pages_of(L) - blk * 8);  // pages of this block that exist
   const int32_t* bt = block_table + (long long)b * max_pages;
   const InT* src = isv ? vsrc : ksrc;
   __shared__ float red[2][NW];

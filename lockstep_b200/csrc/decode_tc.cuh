@@ -137,8 +137,8 @@ __device__ __forceinline__ void decode_plan(const int32_t* seq_lens, int B, int 
     int nb = 0;
     if (i < B) {
       const int L = seq_lens[i];
-      nb = L > 0 ? (L + kKB - 1) / kKB : 0;
-      if (nb > max_blocks || (L + 15) / 16 > max_pages) {
+      nb = L > 0 ? blocks_of(L) : 0;
+      if (nb > max_blocks || pages_of(L) > max_pages) {
         nb = 0;
         atomicOr(err, kDevBadPage);
       } else if (SHARED && L > 0) {
@@ -525,8 +525,8 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_kernel(const Decod
   const bool chan = DH == 2 * kMergeThreads || c0 < DH;  // (dh 64: warp 0 alone has channels)
   const int gq = p.group;
   const int L = p.seq_lens[b];
-  const int nblk = (L + kKB - 1) / kKB;
-  if (L <= 0 || nblk > p.max_blocks || (L + 15) / 16 > p.max_pages) return;   // flagged by the plan
+  const int nblk = blocks_of(L);
+  if (L <= 0 || nblk > p.max_blocks || pages_of(L) > p.max_pages) return;   // flagged by the plan
   if (SHARED && L < p.skip_blocks * kKB) return;
   const int max_part = SHARED ? p.max_part : p.max_blocks;
   const int part0 = SHARED ? p.nfold * kSEG : 0;       // the first block that has partials

@@ -60,7 +60,7 @@ __device__ __forceinline__ void rows_plan(const RowsPlanArgs& p) {
       if (!rows_of(b, n, T0, P)) atomicOr(p.err, kDevPlan);
       else if (n > 0) {
         const int L = p.seq_lens[b];
-        if ((L + kKB - 1) / kKB > p.max_blocks || (L + 15) / 16 > p.max_pages) atomicOr(p.err, kDevBadPage);
+        if (blocks_of(L) > p.max_blocks || pages_of(L) > p.max_pages) atomicOr(p.err, kDevBadPage);
         else nt = (n + 127) / 128;
       }
     }
@@ -97,7 +97,7 @@ __device__ __forceinline__ void rows_plan(const RowsPlanArgs& p) {
     const int t = e - p.tile_off[lo];
     const int kt = T0 / kKB + t;
     int nb = kt + 1;
-    if (kt * kKB < P) nb = max(nb, (P + kKB - 1) / kKB);
+    if (kt * kKB < P) nb = max(nb, blocks_of(P));
     key = kRowsPlanBins - min(nb, kRowsPlanBins);      // longest first
     return make_int4(lo, kt, nb, p.cu_q[lo] + t * 128);
   };

@@ -378,7 +378,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       if (!next_item(rd, it)) continue;
       const int qb = tt & 1;
       const int32_t* bt = p.pg.block_table + (long long)it.b * p.pg.max_pages;
-      const int npages = (it.T + 15) / 16;
+      const int npages = pages_of(it.T);
       auto page_of = [&](int j) -> int {
         const int i = (it.j0 + j) * 8 + lane;
         return lane < 8 && i < npages ? bt[i] : 0;

@@ -26,8 +26,6 @@ struct TablesArgs {
   int* err;
 };
 
-__device__ __forceinline__ int pages_of(int len) { return (len >> 4) + ((len & 15) != 0); }
-
 // exclusive scan of one (tokens, pages) pair a thread over the CTA, 64-bit: (sums before, total)
 __device__ __forceinline__ void scan_pair(long long& a, long long& b, long long& ta, long long& tb, long long (*ws)[32]) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
