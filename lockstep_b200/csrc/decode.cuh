@@ -85,7 +85,8 @@ __device__ __forceinline__ void decode_merge_head(const DecodeArgs& p, int b, in
   const long long bg = (long long)b * p.KVH + g;
   int v0c = 0, evs0 = 0, eh0 = 0;
   if (SINK && L_len > 1) {
-    const int pg = p.block_table[(long long)b * p.max_pages];
+    int pg = p.block_table[(long long)b * p.max_pages];
+    if (pg < 0 || pg >= p.num_pages) pg = 0;             // flagged where its page was loaded
     v0c = (int)p.v8p[((long long)pg * p.KVH + g) * (16 * DH) + c * 16 + 0];
     evs0 = p.ev0[bg];
     eh0 = __ldcg(&p.partM[(bg * p.max_blocks) * gq + h]).z;

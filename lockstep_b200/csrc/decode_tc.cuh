@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_kernel(const Decod
   }
   if (SINK && L > 1 && part0 == 0) {
     int pg = p.block_table[(long long)b * p.max_pages];
-    if (SHARED && (pg < 0 || pg >= p.num_pages)) pg = 0;       // flagged where its page was loaded
+    if (pg < 0 || pg >= p.num_pages) pg = 0;           // flagged where its page was loaded
     const int8_t* v0 = p.v8p + ((long long)pg * p.KVH + g) * (16 * DH);
     if (chan) {
       v0a = (int)v0[c0 * 16];

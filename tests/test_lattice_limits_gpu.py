@@ -60,3 +60,20 @@ def test_the_writers_flag_huge_lengths(dh, length):
         D.build_paged_kv(k.transpose(2, 3).contiguous().transpose(2, 3), v.transpose(2, 3).contiguous().transpose(2, 3), lens,
                          kv.block_table, kv.num_pages, out=kv)
     assert all(torch.equal(a, b) for a, b in zip(keep, (kv.k8p, kv.v8p, kv.ek, kv.ev)))
+
+
+@pytest.mark.parametrize("page", [-1, 10 ** 6, 2 ** 31 - 1, -2 ** 31])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_a_first_page_outside_the_pool_with_the_sink(dh, page):
+    """Key 0's own term reads its value row again in the refold: page 0 stands in there too."""
+    k, v, kv, q = make(dh, sink=True)
+    kv.block_table[1, 0] = 0
+    want = D.decode(q, kv)
+    kv.block_table[1, 0] = page
+    for n in (0, 100):
+        out = torch.zeros_like(q)
+        with pytest.raises(RuntimeError, match="bits 0x4 "):
+            D.decode_shared(q, kv, n, out=out)
+        assert same(out, want)
+    with pytest.raises(RuntimeError, match="bits 0x4 "):
+        D.decode(q, kv)
