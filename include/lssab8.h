@@ -302,7 +302,7 @@ int lssab8_rotate_append(const void* q, const void* k, const void* v, int dtype,
  * page * 16 + row, positions and seq_index; entries of the [cap] arrays past the last token get -1, 0 and -1.
  * pages_used [1]: entries of free_pages taken.  Lengths that do not fit (negative, over 2^30, more tokens than cap,
  * more pages than nfree or max_pages, a missing page in the table) set LSSAB8_DEV_PLAN; the tokens concerned get
- * slot -1.  n <= 16384.  seq_lens may not be before. */
+ * slot -1.  n <= 16384, cap <= 2^30.  What is written may not overlap what is read. */
 int lssab8_step_tables(const int32_t* before, const int32_t* fresh, int n, int32_t* block_table, int64_t table_stride,
                        int max_pages, const int32_t* free_pages, int nfree, int cap, int32_t* query_start_loc,
                        int32_t* seq_lens, int64_t* slot_mapping, int64_t* positions, int32_t* seq_index,

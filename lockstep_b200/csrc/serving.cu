@@ -351,7 +351,7 @@ int lssab8_step_tables(const int32_t* before, const int32_t* fresh, int n, int32
       (cap > 0 && (!slot_mapping || !positions || !seq_index)) || n <= 0 || max_pages <= 0 || table_stride < max_pages ||
       nfree < 0 || cap < 0)
     return kErrArg;
-  if (n > kTblMaxSeqs) return kErrUnsupported;
+  if (n > kTblMaxSeqs || cap > kTblMaxTokens) return kErrUnsupported;
   DevState* ds = nullptr;
   int rc = dev_state(&ds);
   if (rc) return rc;

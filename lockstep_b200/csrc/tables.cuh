@@ -14,6 +14,7 @@ namespace lssab8 {
 
 constexpr int kTblThreads = 1024;
 constexpr int kTblMaxSeqs = 16384;                           // three 4-byte arrays of n in shared memory
+constexpr int kTblMaxTokens = 1 << 30;                       // 32-bit token counters step past it by a grid's threads
 
 struct TablesArgs {
   const int32_t *before, *fresh;      // [n] lengths before the step, new tokens
@@ -99,9 +100,10 @@ __global__ void __launch_bounds__(kTblThreads) step_tables_kernel(const TablesAr
     }
     return lo;
   };
-  for (int e = gid; e < min(page0[p.n], p.nfree); e += gsz) {           // the pages this step takes
-    const int i = find(page0, e);
-    const int j = pages_of(len0[i]) + e - page0[i];
+  const int take = min(page0[p.n], p.nfree);
+  for (long long x = gid; x < take; x += gsz) {              // the pages this step takes (a list may reach 2^31)
+    const int e = (int)x, i = find(page0, e);
+    const int j = pages_of(len0[i]) + (e - page0[i]);
     if (j < p.max_pages) p.table[i * p.table_stride + j] = p.free_pages[e];
     else bad = true;
   }

@@ -11,6 +11,7 @@ from . import attention as _A
 
 PAGE = 16
 MAX_SEQS = 16384
+MAX_TOKENS = 1 << 30
 
 
 @dataclass
@@ -39,7 +40,7 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
 
     block_table [n, max_pages] int32 is updated in place with the new pages, which are the first entries of
     free_pages [F] int32 in sequence order; its other entries stay.  max_tokens: length of the token arrays
-    (at least the step's tokens).  out: tables of an earlier call with the same n and max_tokens, rewritten.
+    (at least the step's tokens, at most 2^30).  out: tables of an earlier call with the same n and max_tokens, rewritten.
     Lengths that do not fit raise RuntimeError (device error 16) when checked."""
     dev = _A._require_cuda(lens, new_tokens, block_table, free_pages)
     n = lens.numel()
@@ -57,8 +58,8 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
     if (step != 1 and width > 1) or (pitch < width and n > 1):
         raise ValueError("block_table rows must be contiguous and apart")
     cap, nfree = int(max_tokens), free_pages.numel()
-    if not 0 <= cap < 1 << 31:
-        raise ValueError("max_tokens must be from 0 to 2^31 - 1")
+    if not 0 <= cap <= MAX_TOKENS:
+        raise ValueError("max_tokens must be from 0 to 2^30")
     lens, new_tokens, free_pages = lens.contiguous(), new_tokens.contiguous(), free_pages.contiguous()
     wrote = [block_table]
     if out is None:

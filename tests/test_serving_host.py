@@ -383,3 +383,19 @@ def test_sequences_on_one_first_page_are_refused(lib):
     step([5, -1, 9, -1, 5], [1, 0, 1, 0, 0], [1, 0, 1, 0, 0])   # idle rows, one over a live sequence's first page
     assert st.slot_of == keep and st.lens[keep[5]] == st.lens[keep[9]] == 2
     assert st.ek[keep[5], 0, 0] == 2 and st.ek[keep[9], 0, 0] == 2 and int((st.ek != 0).sum()) == 2
+
+
+def test_token_counters_stay_in_range(lib):
+    """The kernel's 32-bit counters step by a grid's threads: capacities from which they could wrap are refused, by the
+    host layer and by the library itself."""
+    i32 = torch.zeros(2, dtype=torch.int32)
+    for cap in (2 ** 31 - 1, 2 ** 30 + 1):
+        with pytest.raises(ValueError, match="2\\^30"):
+            P.step_tables(i32, i32.clone(), torch.zeros(2, 4, dtype=torch.int32), i32, cap)
+    assert not lib.names()
+
+
+def test_token_counters_stay_in_range_at_the_c_entry():
+    L, f = _lib.load(), 256
+    call = lambda cap: L.lssab8_step_tables(f, f, 2, f, 4, 4, f, 3, cap, f, f, f, f, f, f, None)     # noqa: E731
+    assert call(2 ** 31 - 1) == call(2 ** 30 + 1) == 2
