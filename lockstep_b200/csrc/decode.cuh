@@ -164,7 +164,6 @@ decode_kernel(const DecodeArgs p) {
   const int nblk = blocks_of(L_len);
   const int first = SHARED ? p.skip_blocks : 0;
   const int nsplit = (nblk - first + p.split_blocks - 1) / p.split_blocks;
-  if (SHARED) pdl_launch_dependents();
   if (L_len <= 0 || split >= nsplit) {
     if (SHARED) pdl_wait();
     return;

@@ -257,8 +257,9 @@ decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_launch_dependents();                             // the refold kernel may queue up behind us
-  pdl_wait();                                          // the plan and the query quantiser are complete
+  if constexpr (!SHARED) pdl_launch_dependents();      // the refold kernel may queue up behind us (SHARED: launched plainly)
+  pdl_wait();                                          // the plan and the query quantiser are complete (SHARED: so is the
+                                                       // shared-prefix kernel, which waited for them)
 
   if (warp == 0) {
     // ================================================================ TMA producer

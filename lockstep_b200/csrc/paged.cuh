@@ -150,7 +150,6 @@ __device__ __forceinline__ void step_plan(const SharedPlanArgs& p) {
 }
 template <typename Plan>
 __global__ void __launch_bounds__(kStepPlanThreads) step_plan_kernel(const Plan plan) {
-  pdl_launch_dependents();
   step_plan(plan);
 }
 // max |x| over a 16-byte vector as a bit pattern, NaN included (a pattern above infinity's)
