@@ -9,6 +9,7 @@ import functools
 
 import torch
 from torch.autograd import forward_ad as _fwd
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -43,8 +44,8 @@ _HERE = _Here()
 
 
 def _on(device):
-    """torch.cuda.device(device), without its cost when the device is current already."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """torch.cuda.device(device), without its cost when the device is current already (device: a CUDA tensor's)."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -115,25 +116,33 @@ def _same_places(a, b):
 
 def _differentiable(*ts):
     """A derivative would have to flow through one of ts: it requires a gradient, or carries a forward-mode tangent."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if _fwd._current_level >= 0 and any(_fwd.unpack_dual(t).tangent is not None for t in ts):
         return True
-    return _fwd._current_level >= 0 and any(_fwd.unpack_dual(t).tangent is not None for t in ts)
+    for t in ts:
+        if t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 def _wrote(*ts):
     """The kernels write through pointers: raise the tensors' versions, so that autograd sees the change as it sees those
     of torch's own in-place operators."""
-    torch.autograd.graph.increment_version(ts)
+    increment_version(ts)
 
 
 def _require_cuda(*ts):
+    i = None
     for t in ts:
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError("LSSA-B8 on B200 needs CUDA tensors (no CPU fallback exists)")
-    i = ts[0].get_device()
-    for t in ts:
-        if t.get_device() != i:
-            raise ValueError("all tensors must be on the same CUDA device")
+        try:
+            d = t.get_device()                               # (-1: not on a GPU)
+        except AttributeError:
+            d = -1
+        if d != i or i is None:
+            if d < 0 or not t.is_cuda:
+                raise ValueError("LSSA-B8 on B200 needs CUDA tensors (no CPU fallback exists)")
+            if i is not None:
+                raise ValueError("all tensors must be on the same CUDA device")
+            i = d
     return ts[0].device
 
 
@@ -409,11 +418,11 @@ def prefill(query, key, value, sink=False, out=None, out_dtype=None, check=True,
     if nbytes == 0:
         raise ValueError("unsupported prefill shape")
     ws = workspace(dev, nbytes)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.check(L.lssab8_prefill(query.data_ptr(), key.data_ptr(), value.data_ptr(), dtype_code(query.dtype), B, H,
-                                    KVH, T, dh, _lib.i64x(query.stride()), _lib.i64x(key.stride()),
-                                    _lib.i64x(value.stride()), int(bool(sink)), out.data_ptr(), dtype_code(out.dtype),
-                                    _lib.i64x(out.stride()), ws.data_ptr(), ws.numel(), _stream_handle(dev)),
+                                    KVH, T, dh, _lib.i64c(query.stride()), _lib.i64c(key.stride()),
+                                    _lib.i64c(value.stride()), int(bool(sink)), out.data_ptr(), dtype_code(out.dtype),
+                                    _lib.i64c(out.stride()), ws.data_ptr(), ws.numel(), _stream_handle(dev)),
                    "lssab8_prefill")
     if check:
         check_device_errors(dev)

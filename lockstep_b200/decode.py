@@ -201,12 +201,12 @@ def decode(q, kv, split_blocks=4, out=None, out_dtype=None, check=True):
     if nbytes == 0:
         raise ValueError("unsupported decode shape")
     ws = _A.workspace(dev, nbytes)
-    with torch.cuda.device(dev):
+    with _A._on(dev):
         _lib.check(L.lssab8_decode(
-            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64x(q.stride()), B, H, kv.KVH, dh, kv.seq_lens.data_ptr(),
+            q.data_ptr(), _A.dtype_code(q.dtype), _lib.i64c(q.stride()), B, H, kv.KVH, dh, kv.seq_lens.data_ptr(),
             kv.block_table.data_ptr(), kv.block_table.shape[1], kv.num_pages, kv.k8p.data_ptr(), kv.v8p.data_ptr(),
             kv.ek.data_ptr(), kv.ev.data_ptr(), kv.ev0.data_ptr(), kv.max_blocks, int(split_blocks), int(kv.sink),
-            out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64x(out.stride()), ws.data_ptr(), ws.numel(),
+            out.data_ptr(), _A.dtype_code(out.dtype), _lib.i64c(out.stride()), ws.data_ptr(), ws.numel(),
             _A._stream_handle(dev)), "lssab8_decode")
     if check:
         _A.check_device_errors(dev)

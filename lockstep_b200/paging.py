@@ -65,10 +65,11 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
     if out is None:
         out = alloc_step_tables(n, cap, dev)
     else:
-        want = alloc_step_tables(n, cap, "meta")
-        for f in StepTables.__dataclass_fields__:
-            t, w = getattr(out, f), getattr(want, f)
-            if t.shape != w.shape or t.dtype != w.dtype or t.device != dev or not t.is_contiguous():
+        i64 = torch.int64
+        for f, t, size, dt in (("query_start_loc", out.query_start_loc, n + 1, i32), ("seq_lens", out.seq_lens, n, i32),
+                               ("slot_mapping", out.slot_mapping, cap, i64), ("positions", out.positions, cap, i64),
+                               ("seq_index", out.seq_index, cap, i32), ("pages_used", out.pages_used, 1, i32)):
+            if t.shape != (size,) or t.dtype != dt or t.device != dev or not t.is_contiguous():
                 raise ValueError("out: tables of another step shape (%s)" % f)
             wrote.append(t)
         ins = [(x.data_ptr(), x.data_ptr() + 4 * size, x) for x, size in (

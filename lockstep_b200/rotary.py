@@ -161,33 +161,45 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
     row.  Slot -1 stores nothing; the other slots must differ (two tokens in one slot leave a mix of both).  Inference
     only: no gradient flows through it."""
     dev = _A._require_cuda(query, key, value, positions, slot_mapping, k_cache, v_cache, plan.freq)
-    if _A._differentiable(query, key, value):
+    if _A._differentiable(query, key, value, k_cache, v_cache):
         raise ValueError("rotate_append has no gradient (use rotate)")
-    query, key, value = query.resolve_neg(), key.resolve_neg(), value.resolve_neg()
-    if _A._differentiable(k_cache, v_cache) or (out is not None and _A._differentiable(out)):
-        raise ValueError("rotate_append has no gradient: out and the caches must not require one")
-    if k_cache.is_neg() or v_cache.is_neg() or (out is not None and out.is_neg()):
-        raise ValueError("out and the caches must not be negative views")
+    qdt, kcdt = query.dtype, k_cache.dtype
+    if qdt is not torch.bfloat16 and (query.is_neg() or key.is_neg() or value.is_neg()):     # (bfloat16 has no complex type)
+        query, key, value = query.resolve_neg(), key.resolve_neg(), value.resolve_neg()
+    if kcdt is not torch.bfloat16 and (k_cache.is_neg() or v_cache.is_neg()):
+        raise ValueError("the caches must not be negative views")
     fresh = out is None
     if fresh:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    elif out.device != dev:
-        raise ValueError("out must be on the query's device")
-    args = _append_args(query.shape, query.stride(), query.dtype, key.shape, key.stride(), key.dtype, value.shape,
-                        value.stride(), value.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape,
-                        v_cache.stride(), v_cache.dtype, out.shape, out.stride(), out.dtype, positions.shape,
-                        positions.dtype, slot_mapping.shape, slot_mapping.dtype, plan.head_dim)
-    dims, qs, ks, vs, pos64, os_, cdt, kcs, vcs, in_place, places = args
+        like = None
+    else:
+        like = out.shape, out.stride(), out.dtype
+        if out.device != dev:
+            raise ValueError("out must be on the query's device")
+        if out.is_neg() or _A._differentiable(out):
+            raise ValueError("out must not be a negative view, nor require a gradient")
+    qp, kp, vp, kcp, vcp = (query.data_ptr(), key.data_ptr(), value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr())
+    args = _append_args(query.shape, query.stride(), qdt, key.shape, key.stride(), key.dtype, value.shape,
+                        value.stride(), value.dtype, k_cache.shape, k_cache.stride(), kcdt, v_cache.shape,
+                        v_cache.stride(), v_cache.dtype, like, positions.shape, positions.dtype, slot_mapping.shape,
+                        slot_mapping.dtype, plan.head_dim)
+    dims, qs, ks, vs, pos64, os_, cdt, kcs, vcs, (nq, nk, nv, nkc, nvc, _), dims_of, in_place = args
     if dims[1] == 0:
         return out
-    _check_places(tuple(zip((query.data_ptr(), key.data_ptr(), value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                             out.data_ptr()), places)), in_place)
-    slot_mapping = slot_mapping.contiguous()
+    op = out.data_ptr()
+    # what is written lies apart from what is read (out may be the query) and from each other: by address ranges,
+    # then exactly where these meet
+    if kcp < vcp + nvc and vcp < kcp + nkc and _A._meet(vcp - kcp, dims_of[3], dims_of[4]):
+        raise ValueError("the caches must lie apart from each other")
+    lo, hi = min(kcp, vcp), max(kcp + nkc, vcp + nvc)
+    if not fresh or (qp < hi and qp + nq > lo) or (kp < hi and kp + nk > lo) or (vp < hi and vp + nv > lo):
+        _check_places((qp, kp, vp, kcp, vcp, op), args[9], dims_of, in_place)
+    if not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.contiguous()
     with _A._on(dev):
         _lib.check(_lib.load().lssab8_rotate_append(
-            query.data_ptr(), key.data_ptr(), value.data_ptr(), *dims, qs, ks, vs, positions.data_ptr(), pos64,
-            positions.stride(0), plan.freq.data_ptr(), plan.factor, plan.rotary_dim, _LAYOUTS[plan.layout],
-            out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), cdt, kcs, vcs, k_cache.shape[0],
+            qp, kp, vp, *dims, qs, ks, vs, positions.data_ptr(), pos64, positions.stride(0), plan.freq.data_ptr(),
+            plan.factor, plan.rotary_dim, _LAYOUTS[plan.layout], op, os_, kcp, vcp, cdt, kcs, vcs, k_cache.shape[0],
             slot_mapping.data_ptr(), _A._stream_handle(dev)), "lssab8_rotate_append")
     if fresh:
         _A._wrote(k_cache, v_cache)
@@ -199,16 +211,17 @@ def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, 
 
 
 @functools.lru_cache(maxsize=1024)
-def _append_args(q, qst, qdt, k, kst, kdt, v, vst, vdt, kc, kcst, kcdt, vc, vcst, vcdt, o, ost, odt, pos, pdt, sl, sdt,
+def _append_args(q, qst, qdt, k, kst, kdt, v, vst, vdt, kc, kcst, kcdt, vc, vcst, vcdt, like, pos, pdt, sl, sdt,
                  head_dim):
     """The checks of rotate_append's shapes, strides and types, and the arguments made from them; kept, since a
-    model's steps repeat them."""
+    model's steps repeat them.  like: out's shape, strides and type (None: a new contiguous one)."""
     if len(q) != 3 or len(k) != 3 or k != v or k[0] != q[0]:
         raise ValueError("query must be [N, H, dh], key and value [N, KVH, dh]")
     if not qdt == kdt == vdt or kcdt != vcdt:
         raise TypeError("query, key and value must share one dtype, and so must the caches")
     N, H, dh = q
     KVH = k[1]
+    o, ost, odt = (q, (H * dh, dh, 1), qdt) if like is None else like
     if dh != head_dim or k[2] != dh:
         raise ValueError("the plan is for head dim %d" % head_dim)
     if len(kc) != 4 or kc != vc or tuple(kc[1:]) != (PAGE, KVH, dh):
@@ -225,21 +238,20 @@ def _append_args(q, qst, qdt, k, kst, kdt, v, vst, vdt, kc, kcst, kcdt, vc, vcst
         raise ValueError("channels must be contiguous")
     if not (_A._apart(ost, o) and _A._apart(kcst, kc) and _A._apart(vcst, vc)):
         raise ValueError("out and the caches must not have elements that share memory")
+    reach, dims_of = zip(*(_A._reach(*x) for x in ((qst, q, qdt), (kst, k, kdt), (vst, v, vdt), (kcst, kc, kcdt),
+                                                   (vcst, vc, vcdt), (ost, o, odt))))
     return ((_A.dtype_code(qdt), N, H, KVH, dh), _lib.i64c(qst[:2]), _lib.i64c(kst[:2]), _lib.i64c(vst[:2]),
             int(pdt == torch.int64), _lib.i64c(ost[:2]), _A.dtype_code(kcdt), _lib.i64c(kcst[:3]), _lib.i64c(vcst[:3]),
-            all(x == y for x, y, n in zip(qst, ost, q) if n > 1),
-            tuple(_A._reach(*x) for x in ((qst, q, qdt), (kst, k, kdt), (vst, v, vdt), (kcst, kc, kcdt), (vcst, vc, vcdt),
-                                          (ost, o, odt))))
+            reach, dims_of, all(x == y for x, y, n in zip(qst, ost, q) if n > 1))
 
 
-def _check_places(at, in_place):
-    """What rotate_append writes (caches, out) lies apart from what it reads, except out on the query itself, and from
-    each other; at: (address, (bytes reached, its dimensions)) of query, key, value, caches, out."""
-    reads, writes = at[:3], at[3:]
-    lo, hi = min(p for p, _ in reads), max(p + n for p, (n, _) in reads)
-    for i, (p, (n, dims)) in enumerate(writes):
-        for j, (p2, (n2, dims2)) in enumerate(writes[:i] + (reads if p < hi and lo < p + n else ())):
-            if p < p2 + n2 and p2 < p + n and not (i == 2 and j == 2 and in_place and p == p2) and \
-                    _A._meet(p2 - p, dims, dims2):
-                raise ValueError("out and the caches must lie apart from the inputs (out may be the query itself) and from "
-                                 "each other")
+def _check_places(at, reach, dims_of, in_place):
+    """query, key, value, key cache, value cache, out, each an address, the bytes reached and its dimensions: the caches
+    and out lie apart from the inputs and out from the caches, except out in the query's own places."""
+    for w, others in ((3, (0, 1, 2)), (4, (0, 1, 2)), (5, (0, 1, 2, 3, 4))):
+        for x in others:
+            d = at[x] - at[w]
+            if -reach[x] < d < reach[w] and not (w == 5 and x == 0 and d == 0 and in_place) and \
+                    _A._meet(d, dims_of[w], dims_of[x]):
+                raise ValueError("out and the caches must lie apart from the inputs (out may be the query) and from each "
+                                 "other")
