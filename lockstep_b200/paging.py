@@ -40,7 +40,8 @@ def step_tables(lens, new_tokens, block_table, free_pages, max_tokens, out=None,
 
     block_table [n, max_pages] int32 is updated in place with the new pages, which are the first entries of
     free_pages [F] int32 in sequence order; its other entries stay.  max_tokens: length of the token arrays
-    (at least the step's tokens, at most 2^30).  out: tables of an earlier call with the same n and max_tokens, rewritten.
+    (at least the step's tokens, at most 2^30).  out: tables of an earlier call with the same n and max_tokens, rewritten
+    (apart from the inputs: lens is not its own seq_lens).
     Lengths that do not fit raise RuntimeError (device error 16) when checked."""
     dev = _A._require_cuda(lens, new_tokens, block_table, free_pages)
     n = lens.numel()

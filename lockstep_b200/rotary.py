@@ -125,9 +125,9 @@ def rotate(x, positions, plan, inverse=False, out=None):
     and shape (any strides; float32, float16, bfloat16).  inverse=True: the transposed map (it undoes
     the rotation when the plan's factor is 1); differentiable in x, the gradient being the other direction
     (forward mode: the tangent is rotated too).
-    out: written instead (out=x rotates in place); not with a gradient.  In a captured graph: torch refuses to capture a
-    backward pass while an eager graph of the same leaf is alive; rotate(g, positions, plan, inverse=True) is the same
-    gradient and needs no graph of the leaf."""
+    out: written instead (out=x rotates in place, else apart from x); not with a gradient.  In a captured graph: torch
+    refuses to capture a backward pass while an eager graph of the same leaf is alive; rotate(g, positions, plan,
+    inverse=True) is the same gradient and needs no graph of the leaf."""
     shape, ps = x.shape, positions.shape
     if len(shape) not in (3, 4) or shape[-1] != plan.head_dim:
         raise ValueError("x must be [B, H, T, %d] or [N, H, %d], got %s" % (plan.head_dim, plan.head_dim, tuple(shape)))
@@ -155,10 +155,10 @@ def rotate(x, positions, plan, inverse=False, out=None):
 
 
 def rotate_append(query, key, value, positions, slot_mapping, k_cache, v_cache, plan, out=None, check=True):
-    """A serving step's new tokens: query [N, H, dh] rotated (returned, or written to out, which may be
-    query), key [N, KVH, dh] rotated and value [N, KVH, dh] stored in k_cache / v_cache [num_pages, 16, KVH, dh]
-    (any page, row and head strides; the cache's own dtype, one rounding) at slot_mapping [N] int64, page * 16 +
-    row.  Slot -1 stores nothing; the other slots must differ (two tokens in one slot leave a mix of both).  Inference
+    """A serving step's new tokens: query [N, H, dh] rotated (returned, or written to out, which may be the query and
+    else lies apart from the inputs), key [N, KVH, dh] rotated and value [N, KVH, dh] stored in k_cache / v_cache
+    [num_pages, 16, KVH, dh], which lie apart from the inputs and each other (any page, row and head strides; the cache's
+    own dtype, one rounding), at slot_mapping [N] int64, page * 16 + row.  Slot -1 stores nothing; the other slots must differ (two tokens in one slot leave a mix of both).  Inference
     only: no gradient flows through it."""
     dev = _A._require_cuda(query, key, value, positions, slot_mapping, k_cache, v_cache, plan.freq)
     if _A._differentiable(query, key, value, k_cache, v_cache):
