@@ -130,6 +130,12 @@ def _wrote(*ts):
     increment_version(ts)
 
 
+def _holds(out, shape, dev):
+    """out has room for rows of this shape, which are written at its start along every dimension."""
+    if out.device != dev or len(out.shape) != len(shape) or any(a < b for a, b in zip(out.shape, shape)):
+        raise ValueError("out must be %s on the query's device" % (tuple(shape),))
+
+
 def _require_cuda(*ts):
     i = None
     for t in ts:
@@ -395,6 +401,8 @@ def prefill(query, key, value, sink=False, out=None, out_dtype=None, check=True,
         raise ValueError("query heads must be a multiple of kv heads")
     if out is None:
         out = torch.empty((B, T, H, dh), dtype=out_dtype or query.dtype, device=dev)
+    else:
+        _holds(out, (B, T, H, dh), dev)
     if mu is not None or qexp != "row" or v_keyshift or b9grid:    # the lattice route
         if qexp not in ("row", "head"):
             raise ValueError(qexp)

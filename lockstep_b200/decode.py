@@ -196,6 +196,8 @@ def decode(q, kv, split_blocks=4, out=None, out_dtype=None, check=True):
         raise ValueError("query does not match the lattice")
     if out is None:
         out = torch.empty((B, H, dh), dtype=out_dtype or q.dtype, device=dev)
+    else:
+        _A._holds(out, q.shape, dev)
     L = _lib.load()
     nbytes = L.lssab8_decode_workspace_size(B, H, kv.KVH, dh, kv.max_blocks)
     if nbytes == 0:

@@ -399,3 +399,20 @@ def test_token_counters_stay_in_range_at_the_c_entry():
     L, f = _lib.load(), 256
     call = lambda cap: L.lssab8_step_tables(f, f, 2, f, 4, 4, f, 3, cap, f, f, f, f, f, f, None)     # noqa: E731
     assert call(2 ** 31 - 1) == call(2 ** 30 + 1) == 2
+
+
+def test_outputs_without_room_are_refused(lib):
+    kv, q = lattice(), torch.zeros(2, 4, 64)
+    x = torch.zeros(1, 4, 200, 64)
+    for out in (torch.zeros(2, 4, 64), torch.zeros(3, 5, 64)):
+        D.decode(q, kv, out=out)
+    A.prefill(x, x[:, :2], x[:, :2], out=torch.zeros(1, 300, 4, 64))
+    n = len(lib.names())
+    for out in (torch.zeros(1, 4, 64), torch.zeros(2, 3, 64), torch.zeros(2, 4, 32), torch.zeros(2 * 4 * 64),
+                torch.zeros(2, 4, 64, device="meta")):
+        with pytest.raises(ValueError):
+            D.decode(q, kv, out=out)
+    for out in (torch.zeros(1, 199, 4, 64), torch.zeros(1, 4, 200, 64), torch.zeros(200, 4, 64)):
+        with pytest.raises(ValueError):
+            A.prefill(x, x[:, :2], x[:, :2], out=out)
+    assert len(lib.names()) == n
